@@ -95,6 +95,17 @@ class Plan(ctypes.Structure):
 
 
 _VP = ctypes.POINTER(ArrayView)
+
+
+class LogitsArgs(ctypes.Structure):
+    """dpx_logits_args"""
+
+    _fields_ = [(n, _VP) for n in ("prompt_tokens", "output_tokens", "prompt_lengths", "output_lengths", "repetition",
+                                   "frequency", "presence")]
+    _fields_ += [(n, ctypes.c_double) for n in ("repetition_value", "frequency_value", "presence_value")]
+    _fields_ += [(n, _VP) for n in ("bias_tokens", "bias_values", "allowed")]
+
+
 _PP = ctypes.POINTER(Plan)
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
@@ -150,6 +161,13 @@ SIGNATURES = {
     "dpx_argreduce": (_i, [_i, _VP, _i, _VP, _vp]),
     "dpx_reduce_plan": (_i, [_i, _VP, _i, _VP, _PP]),
     "dpx_argreduce_plan": (_i, [_i, _VP, _i, _VP, _PP]),
+    "dpx_layer_norm": (_i, [_VP, _VP, _VP, _d, _VP, _VP, _VP, _vp]),
+    "dpx_layer_norm_grad_workspace": (_i64, [_VP]),
+    "dpx_layer_norm_grad": (_i, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _vp, ctypes.c_size_t, _vp]),
+    "dpx_distill_topk_workspace": (_i64, [_VP]),
+    "dpx_distill_topk": (_i, [_VP, _VP, _VP, _d, _VP, _vp, ctypes.c_size_t, _vp]),
+    "dpx_distill_topk_grad": (_i, [_VP, _VP, _VP, _VP, _d, _VP, _VP, _vp, ctypes.c_size_t, _vp]),
+    "dpx_process_logits": (_i, [_VP, ctypes.POINTER(LogitsArgs), _VP, _vp]),
     "dpx_collapse": (_i, [_i, _i, ctypes.POINTER(_i64), ctypes.POINTER(_i64),
                           ctypes.POINTER(_i64), _i]),
 }

@@ -396,6 +396,82 @@ py::object where_call(py::handle cond, py::handle x1, py::handle x2, py::handle 
 }
 
 // ---------------------------------------------------------------------------------------------------------
+// The row operators (layer_norm, distill_topk, process_logits): arrays or None in the order of the C entry points; the
+// Python layer has made the results and laid the arrays out.
+dpx_array_view *view_or_null(py::handle h, const char *what) { return h.is_none() ? nullptr : view_arg(h, what); }
+
+// device memory for one call, from the package's allocator: given back in stream order when the object goes
+struct Workspace {
+    py::object array;
+    void *data = nullptr;
+    size_t bytes = 0;
+    explicit Workspace(int64_t n)
+    {
+        if (n <= 0) return;
+        int64_t shape[1] = {n};
+        dpx_array_view *v;
+        array = fresh_result(Py_None, shape, 1, DPX_UINT8, &v);
+        data = v->data;
+        bytes = (size_t)n;
+    }
+};
+
+void layer_norm(py::handle x, py::handle weight, py::handle bias, double eps, py::handle y, py::handle mean, py::handle rstd)
+{
+    if (int rc = dpx_layer_norm(view_arg(x, "x"), view_or_null(weight, "weight"), view_or_null(bias, "bias"), eps,
+                                view_arg(y, "out"), view_or_null(mean, "mean"), view_or_null(rstd, "rstd"),
+                                stream_of(py::none())))
+        raise_status(rc);
+}
+void layer_norm_grad(py::handle grad, py::handle x, py::handle mean, py::handle rstd, py::handle weight, py::handle dx,
+                     py::handle dweight, py::handle dbias)
+{
+    dpx_array_view *vx = view_arg(x, "x"), *vw = view_or_null(dweight, "dweight");
+    const Workspace ws(vw ? dpx_layer_norm_grad_workspace(vx) : 0);
+    if (int rc = dpx_layer_norm_grad(view_arg(grad, "grad"), vx, view_arg(mean, "mean"), view_arg(rstd, "rstd"),
+                                     view_or_null(weight, "weight"), view_arg(dx, "dx"), vw, view_or_null(dbias, "dbias"),
+                                     ws.data, ws.bytes, stream_of(py::none())))
+        raise_status(rc);
+}
+void distill_topk(py::handle logits, py::handle teacher, py::handle tokens, py::handle weights, double temperature,
+                  py::handle loss, py::handle dlogits)
+{
+    dpx_array_view *vz = view_arg(logits, "logits"), *vt = view_arg(teacher, "teacher_logits"),
+                   *vi = view_arg(tokens, "teacher_tokens"), *vl = view_arg(loss, "loss");
+    const Workspace ws(dpx_distill_topk_workspace(vz));
+    void *s = stream_of(py::none());
+    const int rc = dlogits.is_none()
+                       ? dpx_distill_topk(vz, vt, vi, temperature, vl, ws.data, ws.bytes, s)
+                       : dpx_distill_topk_grad(vz, vt, vi, view_or_null(weights, "weights"), temperature, vl,
+                                               view_arg(dlogits, "dlogits"), ws.data, ws.bytes, s);
+    if (rc) raise_status(rc);
+}
+// penalties: a number or an array
+void process_logits(py::handle logits, py::handle prompt, py::handle prompt_lengths, py::handle output,
+                    py::handle output_lengths, py::handle repetition, py::handle frequency, py::handle presence,
+                    py::handle bias_tokens, py::handle bias_values, py::handle allowed, py::handle out)
+{
+    auto number = [](py::handle h, double *value) -> bool {
+        if (!PyFloat_CheckExact(h.ptr())) return false;
+        *value = PyFloat_AS_DOUBLE(h.ptr());
+        return true;
+    };
+    dpx_logits_args a;
+    a.repetition_value = 1, a.frequency_value = a.presence_value = 0;
+    a.repetition = number(repetition, &a.repetition_value) ? nullptr : view_arg(repetition, "repetition_penalty");
+    a.frequency = number(frequency, &a.frequency_value) ? nullptr : view_arg(frequency, "frequency_penalty");
+    a.presence = number(presence, &a.presence_value) ? nullptr : view_arg(presence, "presence_penalty");
+    a.prompt_tokens = view_or_null(prompt, "prompt_tokens");
+    a.prompt_lengths = view_or_null(prompt_lengths, "prompt_lengths");
+    a.output_tokens = view_or_null(output, "output_tokens");
+    a.output_lengths = view_or_null(output_lengths, "output_lengths");
+    a.bias_tokens = view_or_null(bias_tokens, "bias_tokens");
+    a.bias_values = view_or_null(bias_values, "bias_values");
+    a.allowed = view_or_null(allowed, "allowed");
+    if (int rc = dpx_process_logits(view_arg(logits, "logits"), &a, view_arg(out, "out"), stream_of(py::none()))) raise_status(rc);
+}
+
+// ---------------------------------------------------------------------------------------------------------
 py::cpp_function make_unary(int op, const std::string &name)
 {
     return py::cpp_function(
@@ -545,6 +621,10 @@ PYBIND11_MODULE(_dpx_ext, m)
         },
         py::arg("src"), py::arg("scalar"), py::arg("dst"), py::arg("sycl_queue") = py::none(),
         py::arg("depends") = py::tuple());
+    m.def("layer_norm", &layer_norm);
+    m.def("layer_norm_grad", &layer_norm_grad);
+    m.def("distill_topk", &distill_topk);
+    m.def("process_logits", &process_logits);
     m.def("_array_overlap", [](py::handle a, py::handle b) { return dpx_array_overlap(view_arg(a, "a"), view_arg(b, "b")) != 0; });
     m.def("_same_logical_tensors", [](py::handle a, py::handle b) { return dpx_same_logical(view_arg(a, "a"), view_arg(b, "b")) != 0; });
 }

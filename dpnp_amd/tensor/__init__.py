@@ -65,6 +65,7 @@ from ._reduction import (  # noqa: A004
     reduce_hypot,
     sum,
 )
+from ._row_operators import distill_topk, distill_topk_grad, layer_norm, layer_norm_grad, process_logits
 from ._search_functions import where
 from ._clip import clip
 from ._statistical_functions import mean, std, var

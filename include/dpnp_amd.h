@@ -515,6 +515,57 @@ int dpx_argreduce_plan(int op, const dpx_array_view *src,
                        int trailing_dims_to_reduce, const dpx_array_view *dst,
                        dpx_plan *plan);
 
+/* ---- row operators of language models (no counterpart in the reference, whose users run them as chains of the
+ * calls above over full-size temporaries) -------------------------------------------------------------------------
+ * Operators over the LAST axis; the dims before it are rows and may have any strides, the last axis has unit stride
+ * (DPX_ERR_NOT_IMPLEMENTED otherwise: lay the array out first).  Data is float16, float32 or float64; statistics, sums and
+ * per-row results ("acc" below) are float32, float64 for float64 data; every result is rounded once.  Results do not depend
+ * on the order in which blocks run.  An output may coincide exactly with the input it replaces where that is said, and
+ * overlaps nothing else.  Workspaces are the caller's: 16-byte aligned device memory of the size the _workspace
+ * function gives, with any content, kept until the stream has passed the call, not shared by calls that may overlap. */
+
+/* y = (x - mean) * rstd * weight + bias along the last axis, rstd = 1 / sqrt(variance + eps).  weight, bias: length of the
+ * last axis, x's type (or float32 beside float16 data), each may be NULL.  mean, rstd: acc, the rows' shape, may be NULL.
+ * y may be x. */
+int dpx_layer_norm(const dpx_array_view *x, const dpx_array_view *weight, const dpx_array_view *bias, double eps,
+                   const dpx_array_view *y, const dpx_array_view *mean, const dpx_array_view *rstd, void *stream);
+/* Its gradients from grad (that of y), x and the mean and rstd of the forward pass: dx (may be grad or x), and dweight and
+ * dbias (type of weight, x's without one; both or neither).  The workspace is needed for dweight and dbias only. */
+int64_t dpx_layer_norm_grad_workspace(const dpx_array_view *x);
+int dpx_layer_norm_grad(const dpx_array_view *grad, const dpx_array_view *x, const dpx_array_view *mean,
+                        const dpx_array_view *rstd, const dpx_array_view *weight, const dpx_array_view *dx,
+                        const dpx_array_view *dweight, const dpx_array_view *dbias, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
+/* Distillation from a teacher's top logits: loss (acc, the rows' shape) = T^2 KL(p || q) with p = softmax(teacher_logits /
+ * T) over a row's entries and q = softmax(logits / T).  teacher_logits: logits' type or acc; teacher_tokens: int32 or
+ * int64; both (rows..., K), K <= 2048.  An entry whose token is outside [0, V) is absent; a row with no entry has loss 0. */
+int64_t dpx_distill_topk_workspace(const dpx_array_view *logits);
+int dpx_distill_topk(const dpx_array_view *logits, const dpx_array_view *teacher_logits,
+                     const dpx_array_view *teacher_tokens, double temperature, const dpx_array_view *loss, void *workspace,
+                     size_t workspace_bytes, void *stream);
+/* The loss and dlogits (may be logits) = the gradient of sum(weights * loss); weights: acc, the rows' shape, NULL for ones.
+ * A row of weight 0 and a row with no entry get zeros whatever their logits are. */
+int dpx_distill_topk_grad(const dpx_array_view *logits, const dpx_array_view *teacher_logits,
+                          const dpx_array_view *teacher_tokens, const dpx_array_view *weights, double temperature,
+                          const dpx_array_view *loss, const dpx_array_view *dlogits, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
+/* Arguments of dpx_process_logits; an array that is NULL is not applied. */
+typedef struct dpx_logits_args {
+    const dpx_array_view *prompt_tokens, *output_tokens;   /* (rows..., any) int32 or int64, one type */
+    const dpx_array_view *prompt_lengths, *output_lengths; /* (rows...) int32: entries that count; NULL: all */
+    const dpx_array_view *repetition, *frequency, *presence; /* (rows...) float32; NULL: the value below */
+    double repetition_value, frequency_value, presence_value; /* 1, 0, 0 for none */
+    const dpx_array_view *bias_tokens, *bias_values;       /* (rows..., any) int32 or int64; float32 */
+    const dpx_array_view *allowed;                         /* (rows..., ceil(V / 32)) int32 or uint32: token v's bit is
+                                                              bit v % 32 of word v / 32 */
+} dpx_logits_args;
+/* out (may be logits) = logits with, in this order: tokens of prompt or output divided by repetition where positive,
+ * multiplied where not; frequency * occurrences in the output and, where there are any, presence subtracted; biases added;
+ * tokens whose bit in `allowed` is 0 set to -inf.  Entries outside [0, V) are ignored. */
+int dpx_process_logits(const dpx_array_view *logits, const dpx_logits_args *args, const dpx_array_view *out, void *stream);
+
 /* ---- stride collapsing (exposed for testing) ---------------------------- */
 
 /* Joint collapse of `nops` stride vectors over one shape
