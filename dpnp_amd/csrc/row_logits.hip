@@ -6,10 +6,10 @@
 //   z + the sum of the row's biases for v
 //   -inf                                         if v's bit in the mask is 0
 //
-// Bound by memory for a batch (V logits read and written per row), by latency for one sequence.  A block owns CHUNK
-// neighbouring tokens of a row.  It scans the row's token lists and counts its own tokens in LDS (integer atomics: the
-// counts do not depend on their order), so that no count array of the vocabulary's size exists in memory; then every logit is
-// read, changed and written once.  Arithmetic is float32 (float64 for float64 logits).
+// Bound by memory for a batch (V logits read and written per row), by latency for one sequence.  No count array of the
+// vocabulary's size exists in memory: a block counts the tokens of its part of the vocabulary in LDS (integer atomics: the
+// counts do not depend on their order), and every logit is read, changed and written once.  Arithmetic is float32 (float64
+// for float64 logits).
 #include "row_ops.hpp"
 #include <algorithm>
 
@@ -24,13 +24,14 @@ struct Logits {
     void *out;
     int64_t v;
     int64_t np, no, nb; // entries per row
-    int32_t chunks, tok64, btok64;
+    int32_t chunks, groups; // chunks of a row, and blocks that share them
+    int32_t tok64, btok64;
     double rep0, freq0, pres0; // where no array is given
 };
 
-// a token's word in LDS: the count of its occurrences in the output, two bits above
-constexpr uint32_t SEEN_PROMPT = 1u << 31, HAS_BIAS = 1u << 30, COUNT = HAS_BIAS - 1;
-constexpr int LG_BLOCK = 256;
+// A token's word in LDS: how often the output holds it, whether the prompt does, whether it has a bias.
+constexpr uint32_t COUNT = (1u << 30) - 1, SEEN_PROMPT = 1u << 31, HAS_BIAS = 1u << 30;
+constexpr int BIAS_LIST = 256; // biases of one chunk that are kept in LDS
 
 DPX_D int64_t entry_at(const void *p, int is64, int64_t i)
 {
@@ -44,84 +45,245 @@ DPX_D int64_t entries_of(const void *len, int64_t at, int64_t n)
     return k < 0 ? 0 : k < n ? k : n;
 }
 
-template <class T, int CHUNK> __global__ __launch_bounds__(LG_BLOCK) void logits_kernel(Logits a)
+// A row's token list, looked through by a block once per chunk (tokens are below 2^30, entries too: everything is an int).
+// HELD packs of 16 bytes per thread are read once and stay in registers; what lies beyond is read again for every chunk.
+template <int BT> struct TokenScan {
+    static constexpr int HELD = BT >= 512 ? 1 : 2;
+    const char *list = nullptr;
+    bool is64;
+    int k = 0, whole = 0; // entries that count; whole packs of the list (the entries beyond them are read one by one)
+    u32x4 raw[HELD];
+    int held[4 * HELD];
+    // sent for before the row's length is known: the list's extent bounds it
+    DPX_D void send(const void *p, int is64_, int64_t at, int64_t extent)
+    {
+        is64 = is64_ != 0;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) raw[h] = u32x4{~0u, ~0u, ~0u, ~0u};
+        if (!p) return;
+        list = (const char *)p + at * (is64 ? 8 : 4);
+        whole = (int)(extent / (is64 ? 2 : 4));
+#pragma unroll
+        for (int h = 0; h < HELD; ++h)
+            if ((int)threadIdx.x + h * BT < whole) raw[h] = load_words16<false>(list + ((int)threadIdx.x + h * BT) * 16);
+    }
+    static constexpr int NONE = 0x7fffffff;
+    static DPX_D int narrow(int64_t t) { return t < 0 || t > 0x3fffffff ? NONE : (int)t; }
+    DPX_D void arrived(int64_t entries)
+    {
+        if (!list) return;
+        k = (int)entries;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            const int left = k - ((int)threadIdx.x + h * BT) * (is64 ? 2 : 4);
+            int *t = held + 4 * h;
+            if (is64) {
+                t[0] = narrow((int64_t)(((uint64_t)raw[h][1] << 32) | raw[h][0]));
+                t[1] = narrow((int64_t)(((uint64_t)raw[h][3] << 32) | raw[h][2]));
+                t[2] = t[3] = NONE;
+            }
+            else
+#pragma unroll
+                for (int c = 0; c < 4; ++c) t[c] = narrow((int)raw[h][c]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) t[c] = c < left ? t[c] : NONE;
+        }
+    }
+    // calls f(t - begin) for the entries t in [begin, begin + n)
+    template <class F> DPX_D void take(int begin, int n, F f) const
+    {
+        if (!list) return;
+        auto one = [&](int token) {
+            const uint32_t t = (uint32_t)token - (uint32_t)begin;
+            if (t < (uint32_t)n) f((int)t);
+        };
+#pragma unroll
+        for (int c = 0; c < 4 * HELD; ++c) one(held[c]);
+        const int packs = whole < HELD * BT ? whole : HELD * BT, c = is64 ? 2 : 4; // what the registers hold
+        for (int i = packs * c + (int)threadIdx.x; i < k; i += BT)
+            one(narrow(is64 ? ((const int64_t *)list)[i] : (int64_t)((const int32_t *)list)[i]));
+    }
+};
+
+// A block takes a run of a row's chunks of CHUNK neighbouring tokens, one after the other, the next chunk's logits on their
+// way.  Per chunk the lists' tokens are counted in LDS words; then every thread looks at the words of its own packs, and
+// where there are any, puts the pack into its place in LDS and processes the named tokens there one by one (a wave runs as
+// many rounds as the most named pack of its lanes has, mostly one), clears the words, and stores the pack.
+template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void logits_kernel(Logits a)
 {
     using A = acc_of<T>;
-    constexpr int E = 16 / (int)sizeof(T);
-    __shared__ uint32_t word[CHUNK];
-    const int64_t row = blockIdx.x / (uint32_t)a.chunks;
-    const int64_t begin = (int64_t)(blockIdx.x - (uint32_t)row * (uint32_t)a.chunks) * CHUNK;
-    const int n = (int)(begin + CHUNK < a.v ? CHUNK : a.v - begin);
-    for (int i = threadIdx.x * 4; i < CHUNK; i += LG_BLOCK * 4) *(u32x4 *)(word + i) = u32x4{0, 0, 0, 0};
-    __syncthreads();
-    if (a.prompt) {
-        const int64_t at = a.map.template off<L_PROMPT>(row), k = entries_of(a.plen, a.map.template off<L_PLEN>(row), a.np);
-        for (int64_t i = threadIdx.x; i < k; i += LG_BLOCK) {
-            const int64_t t = entry_at(a.prompt, a.tok64, at + i) - begin;
-            if (t >= 0 && t < n) atomicOr(&word[t], SEEN_PROMPT);
-        }
-    }
-    if (a.output) {
-        const int64_t at = a.map.template off<L_OUTPUT>(row), k = entries_of(a.olen, a.map.template off<L_OLEN>(row), a.no);
-        for (int64_t i = threadIdx.x; i < k; i += LG_BLOCK) {
-            const int64_t t = entry_at(a.output, a.tok64, at + i) - begin;
-            if (t >= 0 && t < n) atomicAdd(&word[t], 1u);
-        }
-    }
+    constexpr int E = 16 / (int)sizeof(T), PPT = CHUNK / (BT * E);
+    static_assert(PPT * BT * E == CHUNK && CHUNK % 32 == 0 && CHUNK <= 65536);
+    __shared__ __attribute__((aligned(16))) uint32_t word[CHUNK];
+    __shared__ __attribute__((aligned(16))) T value[BT * E]; // a pack per thread
+    __shared__ int bias_at[BIAS_LIST];
+    __shared__ float bias[BIAS_LIST];
+    __shared__ int bias_count;
+    const int64_t row = blockIdx.x / (uint32_t)a.groups;
+    const int group = (int)(blockIdx.x - (uint32_t)row * (uint32_t)a.groups), tid = (int)threadIdx.x, v = (int)a.v;
+    int chunk = (int)((int64_t)group * a.chunks / a.groups);
+    const int stop = (int)((int64_t)(group + 1) * a.chunks / a.groups);
+    const T *z = (const T *)a.z + a.map.template off<L_Z>(row);
+    T *out = (T *)a.out + a.map.template off<L_OUT>(row);
+    const uint8_t *mask = a.mask ? (const uint8_t *)((const uint32_t *)a.mask + a.map.template off<L_MASK>(row)) : nullptr;
+    // the packs are laid so that they are aligned in `out` (rows of an odd length start anywhere): the first one starts `shift`
+    // elements before the row
+    const int shift = (int)((uintptr_t)out / sizeof(T)) & (E - 1);
+    // a pack's mask bits: two bytes at once, the last ones of the row at most (positions below 0 or past v are not asked for)
+    const int mask_last = (v + 31) / 32 * 4 - 2;
+    auto mask_byte = [&](int i) { return i >> 3 < mask_last ? i >> 3 : mask_last; };
+    auto allowed = [&](int i) { return (mask[i >> 3] >> (i & 7)) & 1; };
+    TokenScan<BT> prompt, output;
+    prompt.send(a.prompt, a.tok64, a.map.template off<L_PROMPT>(row), a.np);
+    output.send(a.output, a.tok64, a.map.template off<L_OUTPUT>(row), a.no);
+    // the last wave looks after the biases
+    const int lane = tid - (BT - 64), nb = (int)a.nb;
     const int64_t bt = a.btok ? a.map.template off<L_BTOK>(row) : 0, bv = a.btok ? a.map.template off<L_BVAL>(row) : 0;
-    if (a.btok)
-        for (int64_t i = threadIdx.x; i < a.nb; i += LG_BLOCK) {
-            const int64_t t = entry_at(a.btok, a.btok64, bt + i) - begin;
-            if (t >= 0 && t < n) atomicOr(&word[t], HAS_BIAS);
+    auto bias_token = [&](int k) { return TokenScan<BT>::narrow(entry_at(a.btok, a.btok64, bt + k)); };
+    auto bias_value = [&](int k) { return ((const float *)a.bval)[bv + k]; };
+    int b_token = TokenScan<BT>::NONE;
+    float b_value = 0;
+    if (a.btok && lane >= 0 && lane < nb) {
+        b_token = bias_token(lane);
+        b_value = bias_value(lane);
+    }
+    auto fetch = [&](int c, pack<T, E>(&x)[PPT], uint32_t(&ok)[PPT]) {
+#pragma unroll
+        for (int j = 0; j < PPT; ++j) {
+            const int i = c * CHUNK - shift + (j * BT + tid) * E;
+            if (i >= 0 && i + E <= v) {
+                x[j] = load_pack<T, E>(z + i);
+                if (mask) ok[j] = load_pack<uint16_t, 1, false>((const uint16_t *)(mask + mask_byte(i))).v[0];
+            }
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[j].v[e] = i + e >= 0 && i + e < v ? z[i + e] : (T)0;
         }
+    };
+    pack<T, E> x[PPT], x2[PPT];
+    uint32_t ok[PPT], ok2[PPT];
+    fetch(chunk, x, ok);
+    const bool lists = a.prompt || a.output || a.btok;
     const A rep = a.rep ? (A)((const float *)a.rep)[a.map.template off<L_REP>(row)] : (A)a.rep0;
     const A freq = a.freq ? (A)((const float *)a.freq)[a.map.template off<L_FREQ>(row)] : (A)a.freq0;
     const A pres = a.pres ? (A)((const float *)a.pres)[a.map.template off<L_PRES>(row)] : (A)a.pres0;
-    const uint32_t *mask = a.mask ? (const uint32_t *)a.mask + a.map.template off<L_MASK>(row) : nullptr;
-    __syncthreads();
-    const T *z = (const T *)a.z + a.map.template off<L_Z>(row) + begin;
-    T *out = (T *)a.out + a.map.template off<L_OUT>(row) + begin;
-    auto change = [&](T z0, int i) -> T {
-        const uint32_t w = word[i];
-        T r = z0;
-        if (w) {
-            A x = (A)z0;
-            if (w & (SEEN_PROMPT | COUNT)) x = x > 0 ? x / rep : x * rep;
-            const uint32_t said = w & COUNT;
-            if (said) x = (x - freq * (A)said) - pres;
-            if (w & HAS_BIAS) { // the biases of this token added up in their order, then to the logit
-                A s = 0;
-                for (int64_t k = 0; k < a.nb; ++k)
-                    if (entry_at(a.btok, a.btok64, bt + k) == begin + i) s += (A)((const float *)a.bval)[bv + k];
-                x += s;
+    prompt.arrived(entries_of(a.plen, a.map.template off<L_PLEN>(row), a.np));
+    output.arrived(entries_of(a.olen, a.map.template off<L_OLEN>(row), a.no));
+    if (lists)
+        for (int i = tid * 4; i < CHUNK; i += BT * 4) *(u32x4 *)(word + i) = u32x4{0, 0, 0, 0};
+    T *mine = value + tid * E;
+    for (; chunk < stop; ++chunk) {
+        const int begin = chunk * CHUNK - shift, n = v - begin < CHUNK ? v - begin : CHUNK;
+        if (chunk + 1 < stop) fetch(chunk + 1, x2, ok2);
+        if (lists) {
+            __syncthreads(); // the words are clear
+            prompt.take(begin, n, [&](int t) { atomicOr(&word[t], SEEN_PROMPT); });
+            output.take(begin, n, [&](int t) { atomicAdd(&word[t], 1u); });
+            if (a.btok && lane >= 0) { // the chunk's biases, listed in their order
+                int count = 0;
+                for (int k = lane; k - lane < nb; k += 64) {
+                    int token = b_token;
+                    float value = b_value;
+                    if (k >= 64) {
+                        token = k < nb ? bias_token(k) : TokenScan<BT>::NONE;
+                        value = k < nb ? bias_value(k) : 0.0f;
+                    }
+                    const uint32_t t = (uint32_t)token - (uint32_t)begin;
+                    const bool in = t < (uint32_t)n;
+                    const uint64_t who = __builtin_amdgcn_ballot_w64(in);
+                    const int at = count + __builtin_popcountll(who & (((uint64_t)1 << lane) - 1));
+                    if (in) {
+                        atomicOr(&word[t], HAS_BIAS);
+                        if (at < BIAS_LIST) {
+                            bias_at[at] = (int)t;
+                            bias[at] = value;
+                        }
+                    }
+                    count += __builtin_popcountll(who);
+                }
+                if (lane == 0) bias_count = count;
             }
-            r = (T)x;
+            __syncthreads();
         }
-        if (mask && !((mask[(begin + i) >> 5] >> (i & 31)) & 1)) r = (T)(-__builtin_inff());
-        return r;
-    };
-    for (int i = threadIdx.x * E; i < n; i += LG_BLOCK * E) {
-        if (i + E <= n) {
-            pack<T, E> x = load_pack<T, E>(z + i);
 #pragma unroll
-            for (int e = 0; e < E; ++e) x.v[e] = change(x.v[e], i + e);
-            store_pack<T, E>(out + i, x);
+        for (int j = 0; j < PPT; ++j) {
+            const int i = (j * BT + tid) * E;
+            if (lists) {
+                uint32_t w[E], any = 0;
+                load_vals<E, false>(word + i, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) any |= w[e];
+                if (any) {
+                    uint32_t named = 0;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) named |= (w[e] != 0) << e;
+                    *(pack<T, E> *)mine = x[j];
+                    for (; named; named &= named - 1) {
+                        const int e = __builtin_ctz(named);
+                        const uint32_t word_e = word[i + e];
+                        A r = (A)mine[e];
+                        if (word_e & (SEEN_PROMPT | COUNT)) r = r > 0 ? r / rep : r * rep;
+                        const uint32_t said = word_e & COUNT;
+                        if (said) r = (r - freq * (A)said) - pres;
+                        if (word_e & HAS_BIAS) { // the biases of this token added up in their order, then to the logit
+                            A s = 0;
+                            if (bias_count <= BIAS_LIST) {
+                                for (int k = 0; k < bias_count; ++k)
+                                    if (bias_at[k] == i + e) s += (A)bias[k];
+                            }
+                            else
+                                for (int k = 0; k < nb; ++k)
+                                    if (bias_token(k) == begin + i + e) s += (A)bias_value(k);
+                            r += s;
+                        }
+                        mine[e] = (T)r;
+                        word[i + e] = 0;
+                    }
+                    x[j] = *(const pack<T, E> *)mine;
+                }
+            }
+            const int g = begin + i;
+            if (g >= 0 && i + E <= n) {
+                if (mask) {
+                    const uint32_t bits = ok[j] >> (g - 8 * mask_byte(g));
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[j].v[e] = (bits >> e) & 1 ? x[j].v[e] : (T)(-__builtin_inff());
+                }
+                store_pack<T, E>(out + g, x[j]);
+            }
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (g + e >= 0 && i + e < n) out[g + e] = !mask || allowed(g + e) ? x[j].v[e] : (T)(-__builtin_inff());
+            x[j] = x2[j];
+            ok[j] = ok2[j];
         }
-        else
-            for (int e = i; e < n; ++e) out[e] = change(z[e], e);
     }
 }
 
 constexpr int64_t MAX_GRID = 0x7fffffff;
-constexpr int LG_CHUNK = 4096; // a multiple of 32: a chunk starts at a whole word of the mask
 
-template <class T> int logits_launch(Logits &a, hipStream_t s)
+template <class T, int CHUNK, int BT> int logits_launch_as(Logits &a, int64_t slots, hipStream_t s)
 {
-    a.chunks = (int32_t)((a.v + LG_CHUNK - 1) / LG_CHUNK);
-    if (a.map.rows * a.chunks > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, "process_logits: too many rows for one launch");
-    hipLaunchKernelGGL((logits_kernel<T, LG_CHUNK>), dim3((unsigned)(a.map.rows * a.chunks)), dim3(LG_BLOCK), 0, s, a);
+    a.chunks = (int32_t)((a.v + 16 / sizeof(T) - 1 + CHUNK - 1) / CHUNK); // packs may start before the row
+    a.groups = (int32_t)std::max<int64_t>(1, std::min<int64_t>(a.chunks, slots / a.map.rows));
+    if (a.map.rows * a.groups > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, "process_logits: too many rows for one launch");
+    hipLaunchKernelGGL((logits_kernel<T, CHUNK, BT>), dim3((unsigned)(a.map.rows * a.groups)), dim3(BT), 0, s, a);
     const hipError_t rc = hipGetLastError();
     return rc == hipSuccess ? DPX_OK : fail_hip(rc, "process_logits launch");
+}
+// Chunks and blocks.  With many rows: 8192 tokens by 512 threads (float64: 2048, whose registers spill beyond), three blocks a
+// CU that share out each row's chunks and keep the next chunk's logits in flight while they count (256 rows of 100003
+// float16, lists of 1800 and 700 tokens, 50 biases, mask: 28.9 us; a block per chunk, which reads the lists anew and has
+// nothing in flight meanwhile: 38.7; 4096 tokens by 256 threads: 30.3).  Without lists there is nothing to keep: a block per
+// chunk streams better (mask alone 22.8 against 24.8 us).  With few rows small chunks, so that the row is spread over the CUs.
+template <class T> int logits_launch(Logits &a, hipStream_t s)
+{
+    constexpr int E = 16 / (int)sizeof(T), CHUNK = sizeof(T) == 8 ? 2048 : 8192;
+    const int64_t cus = device_cus(), many = (int64_t)1 << 40;
+    const bool lists = a.prompt || a.output || a.btok;
+    if (a.map.rows * ((a.v + CHUNK - 1) / CHUNK) >= cus * 2) return logits_launch_as<T, CHUNK, 512>(a, lists ? cus * 3 : many, s);
+    return logits_launch_as<T, 256 * E, 256>(a, many, s);
 }
 
 int process_logits_call(const dpx_array_view *logits, const dpx_logits_args *g, const dpx_array_view *out, hipStream_t stream)
@@ -162,8 +324,9 @@ int process_logits_call(const dpx_array_view *logits, const dpx_logits_args *g, 
         return fail(DPX_ERR_BAD_ARGUMENT, "process_logits: repetition_penalty must be a positive number");
     for (double v : {g->frequency ? 0.0 : g->frequency_value, g->presence ? 0.0 : g->presence_value})
         if (!(v >= -1e30 && v <= 1e30)) return fail(DPX_ERR_BAD_ARGUMENT, "process_logits: penalties must be finite numbers");
-    // a count has 30 bits of its word
-    if (a.no > (int64_t)COUNT) return fail(DPX_ERR_BAD_ARGUMENT, "process_logits: output_tokens has too many entries per row");
+    // (a count has 30 bits of its word; positions are ints)
+    for (int64_t k : {a.v, a.np, a.no, a.nb})
+        if (k >= (1 << 30)) return fail(DPX_ERR_BAD_ARGUMENT, "process_logits: a last axis is too long");
     if (a.map.rows == 0 || a.v == 0) return DPX_OK;
     a.z = p[L_Z], a.out = p[L_OUT], a.prompt = p[L_PROMPT], a.output = p[L_OUTPUT], a.plen = p[L_PLEN], a.olen = p[L_OLEN];
     a.rep = p[L_REP], a.freq = p[L_FREQ], a.pres = p[L_PRES], a.btok = p[L_BTOK], a.bval = p[L_BVAL], a.mask = p[L_MASK];

@@ -449,8 +449,13 @@ def test_logits_long_history_and_many_rows(dt):
     d["plen"][:] = [5003, 17]
     d["olen"][:] = [40000, 39999]
     check_logits(z, d)
-    z, d = logits_data(rng, 300, 260, dt)
+    z, d = logits_data(rng, 300, 260, dt, nb=700)  # more biases in a block's part of the vocabulary than it lists
     check_logits(z, d)
+    for r, v in ((600, 260), (400, 20011), (70, 70003)):  # many rows: blocks that go through several parts of a row
+        z, d = logits_data(rng, r, v, dt, 50, 30, nb=20)
+        d["prompt"][:, 20:] = np.where(d["prompt"][:, 20:] >= 0, rng.integers(0, v, (r, 30)), -1)
+        check_logits(z, d)
+    check_logits(z, {"allowed": d["allowed"]})  # ... and without lists
     z, d = logits_data(rng, 1, 131072, dt, 700, 300)
     check_logits(z, d)
 
