@@ -83,6 +83,7 @@ int row_validate(const char *fn, int nargs, const RowArg *args, int64_t &rows, i
         shape[d] = first->shape[d];
         for (int k = 0; k < nargs; ++k) s[k][d] = args[k].v ? args[k].v->strides[d] : 0;
     }
+    if (rows > 0x7fffffff) return bad(DPX_ERR_BAD_ARGUMENT, fn, "more than 2147483647 rows");
     if (rows == 0) {
         nd = 0;
         return DPX_OK;

@@ -4,8 +4,16 @@
 //   backward   h = (x - m) s,  g = dy w,  dx = s (g - mean(g) - h mean(g h)),  dw = sum_rows dy h,  db = sum_rows dy
 //
 // Both are bound by memory: 2 and 3 rows of traffic.  A row is read once and stays in registers between the statistics
-// and the result, so G lanes of a wave or a whole block own it and each lane holds PPL packs of E elements of it.
-// float16 and float32 rows are computed in float32, float64 rows in float64; every result is rounded once, at its store.
+// and the result: G lanes of a wave or a whole block own it, each lane holds PPL packs of E elements of it, and the blocks
+// walk down the rows with the next row on its way, so that weights are read (and the backward's column sums kept) in
+// registers.  float16 and float32 rows are computed in float32, float64 rows in float64; every result is rounded once, at
+// its store.
+//
+// Measured (rocprofv3): forward of 16384 x 4096 float16 with float32 parameters 47 us (5.7 TB/s; one block per row that
+// reads the weights anew 60 us, one wave per row 56), 20011 x 1001 float32 29.5 us (5.4 TB/s: rows off the 16-byte grid);
+// backward of 16384 x 4096 float16 78 us + 4.7 for the fold of the column sums (5.2 TB/s), 2049 x 10007 float32 53 + 6.5.
+// The backward's time does not change with the prefetch distance (0, 1, 2 rows), the threads per row (256 to 1024) or its
+// arithmetic (9 against 16 instructions per element): it is what three streams of persistent blocks reach here.
 #include "row_ops.hpp"
 #include <algorithm>
 
@@ -35,27 +43,39 @@ template <int E, int G> struct PackAt {
     }
 };
 
+DPX_D float row_fma(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+DPX_D double row_fma(double a, double b, double c) { return __builtin_fma(a, b, c); }
 DPX_D float row_sqrt(float v) { return __builtin_sqrtf(v); }
 DPX_D double row_sqrt(double v) { return __builtin_sqrt(v); }
 
-// Sums over the G lanes of a row: inside a wave by DPP, over the waves of a block through LDS (one barrier; `slot`
-// alternates so that the next sum needs none before it writes).
-template <int G, int BT, int NV, class A> DPX_D void row_sums(A (&v)[NV], A (*lds)[BT / 64][NV], int slot)
+// Sums over the G lanes of a row.  Up to 64 lanes: by DPP.  A block: each row of 16 lanes leaves its sums in LDS, and after a
+// barrier every row of 16 lanes reads all of them, BT / 256 per lane, and adds them up by DPP again.  `slot` alternates, so
+// that the next sum needs no barrier before it writes.
+template <int NV, class A> struct alignas(NV * sizeof(A)) SumPart {
+    A v[NV];
+};
+template <int G, int BT, int NV, class A> DPX_D void row_sums(A (&v)[NV], SumPart<NV, A> (*lds)[BT / 16], int slot)
 {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = lanes_fold<(G > 64 ? 64 : G)>(v[i], SumOp{});
+    for (int i = 0; i < NV; ++i) v[i] = lanes_fold<(G > 64 ? 16 : G)>(v[i], SumOp{});
     if constexpr (G > 64) {
-        const int wave = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0)
+        if ((threadIdx.x & 15) == 0) {
+            SumPart<NV, A> p;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) lds[slot][wave][i] = v[i];
+            for (int i = 0; i < NV; ++i) p.v[i] = v[i];
+            lds[slot][threadIdx.x >> 4] = p;
+        }
         __syncthreads();
+        constexpr int PER = BT / 256; // (blocks that share a row have 256 threads or more)
+        SumPart<NV, A> p[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) p[k] = lds[slot][(threadIdx.x & 15) * PER + k];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            A s = lds[slot][0][i];
+            v[i] = p[0].v[i];
 #pragma unroll
-            for (int k = 1; k < BT / 64; ++k) s += lds[slot][k][i];
-            v[i] = s;
+            for (int k = 1; k < PER; ++k) v[i] += p[k].v[i];
+            v[i] = lanes_fold<16>(v[i], SumOp{});
         }
     }
 }
@@ -64,52 +84,74 @@ template <int G, int BT, int NV, class A> DPX_D void row_sums(A (&v)[NV], A (*ld
 template <class T, class W, int E, int PPL, int G, int BT> __global__ __launch_bounds__(BT) void norm_fwd_kernel(NormFwd a)
 {
     using A = acc_of<T>;
-    __shared__ A lds[2][BT / 64][1];
-    const int li = threadIdx.x % G;
-    const int64_t row = (int64_t)blockIdx.x * (BT / G) + threadIdx.x / G;
-    if (row >= a.map.rows) return;
-    const T *x = (const T *)a.x + a.map.template off<0>(row);
-    const int64_t n = a.n;
-    A v[PPL][E];
-#pragma unroll
-    for (int j = 0; j < PPL; ++j) load_vals<E, true>(x + PackAt<E, G>(n, li, j).base, v[j]);
+    __shared__ SumPart<1, A> lds[4][BT / 16];
+    constexpr int NG = BT / G;
+    const int li = NG > 1 ? threadIdx.x % G : threadIdx.x, gi = NG > 1 ? threadIdx.x / G : 0; // (one row a block: uniform)
+    const int64_t n = a.n, rows = a.map.rows, step = (int64_t)gridDim.x * NG;
     const PackAt<E, G> last(n, li, PPL - 1); // only a lane's last pack can be partial
-    A s[1] = {0};
+    const A inv_n = A(1) / (A)n;
+    // the weights, and the next row, stay in registers as long as they fit
+    constexpr bool HOLD = BT < 1024 || PPL <= (E == 8 ? 3 : 5);
+    auto weights = [&](int j, A(&w)[E], A(&b)[E]) {
+        const int64_t base = PackAt<E, G>(n, li, j).base;
 #pragma unroll
-    for (int j = 0; j < PPL; ++j)
+        for (int e = 0; e < E; ++e) w[e] = 1, b[e] = 0;
+        if (a.w) load_vals<E, false>((const W *)a.w + base, w);
+        if (a.b) load_vals<E, false>((const W *)a.b + base, b);
+    };
+    A w[HOLD ? PPL : 1][E], b[HOLD ? PPL : 1][E];
+    if constexpr (HOLD)
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[0] += (j < PPL - 1 || e >= last.skip) ? v[j][e] : A(0);
-    row_sums<G, BT>(s, lds, 0);
-    const A mean = s[0] / (A)n;
-    s[0] = 0;
+        for (int j = 0; j < PPL; ++j) weights(j, w[j], b[j]);
+    struct Row {
+        pack<T, E> x[PPL];
+        T *y;
+    };
+    auto fetch = [&](int64_t row, Row &r) {
+        const T *x = (const T *)a.x + a.map.template off<0>(row);
+        r.y = (T *)a.y + a.map.template off<1>(row);
 #pragma unroll
-    for (int j = 0; j < PPL; ++j)
+        for (int j = 0; j < PPL; ++j) r.x[j] = load_pack<T, E>(x + PackAt<E, G>(n, li, j).base);
+    };
+    int64_t row = (int64_t)blockIdx.x * NG + gi;
+    Row r;
+    if (row < rows) fetch(row, r);
+    int slot = 0;
+    for (; row < rows; row += step, slot ^= 2) {
+        Row next;
+        if constexpr (HOLD) fetch(row + step < rows ? row + step : row, next);
+        A s[1] = {0};
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            v[j][e] -= mean;
-            s[0] += (j < PPL - 1 || e >= last.skip) ? v[j][e] * v[j][e] : A(0);
+        for (int j = 0; j < PPL; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) s[0] += (j < PPL - 1 || e >= last.skip) ? (A)r.x[j].v[e] : A(0);
+        row_sums<G, BT>(s, lds, slot);
+        const A mean = s[0] * inv_n;
+        s[0] = 0;
+#pragma unroll
+        for (int j = 0; j < PPL; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const A d = (j < PPL - 1 || e >= last.skip) ? (A)r.x[j].v[e] - mean : A(0);
+                s[0] = row_fma(d, d, s[0]);
+            }
+        row_sums<G, BT>(s, lds, slot + 1);
+        const A rstd = A(1) / row_sqrt(s[0] * inv_n + (A)a.eps);
+        auto centred = [&](T x) { return ((A)x - mean) * rstd; };
+#pragma unroll
+        for (int j = 0; j < PPL; ++j) {
+            A o[E];
+            if constexpr (!HOLD) weights(j, w[0], b[0]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = row_fma(centred(r.x[j].v[e]), w[HOLD ? j : 0][e], b[HOLD ? j : 0][e]);
+            store_vals<E, true>(r.y + PackAt<E, G>(n, li, j).base, o);
         }
-    row_sums<G, BT>(s, lds, 1);
-    const A rstd = A(1) / row_sqrt(s[0] / (A)n + (A)a.eps);
-    T *y = (T *)a.y + a.map.template off<1>(row);
-#pragma unroll
-    for (int j = 0; j < PPL; ++j) {
-        const PackAt<E, G> at(n, li, j);
-        if (at.skip >= E) continue;
-        A w[E], b[E], o[E];
-        if (a.w) load_vals<E, false>((const W *)a.w + at.base, w);
-        if (a.b) load_vals<E, false>((const W *)a.b + at.base, b);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            o[e] = v[j][e] * rstd;
-            if (a.w) o[e] *= w[e];
-            if (a.b) o[e] += b[e];
+        if (li == 0) {
+            if (a.mean) ((A *)a.mean)[a.map.template off<2>(row)] = mean;
+            if (a.rstd) ((A *)a.rstd)[a.map.template off<3>(row)] = rstd;
         }
-        store_vals<E, true>(y + at.base, o);
-    }
-    if (li == 0) {
-        if (a.mean) ((A *)a.mean)[a.map.template off<2>(row)] = mean;
-        if (a.rstd) ((A *)a.rstd)[a.map.template off<3>(row)] = rstd;
+        if constexpr (HOLD) r = next;
+        else if (row + step < rows) fetch(row + step, r);
     }
 }
 
@@ -118,7 +160,7 @@ template <class T, class W, int E, int PPL, int G, int BT> __global__ __launch_b
 template <class T, class W, int BT> __global__ __launch_bounds__(BT) void norm_fwd_long_kernel(NormFwd a)
 {
     using A = acc_of<T>;
-    __shared__ A lds[2][BT / 64][1];
+    __shared__ SumPart<1, A> lds[2][BT / 16];
     const int64_t row = blockIdx.x, n = a.n;
     const T *x = (const T *)a.x + a.map.template off<0>(row);
     A s[1] = {0};
@@ -156,13 +198,15 @@ struct NormBwd {
 
 // A block (or each of its groups of G lanes) walks down the rows, gridDim apart, and keeps its columns' sums for dw and db in
 // registers; at the end they go to the block's slice of the workspace, which norm_grad_fold_kernel adds up in block order.
-template <class T, class W, int E, int PPL, int G, int BT> __global__ __launch_bounds__(BT) void norm_grad_kernel(NormBwd a)
+// AHEAD: the next row is on its way while this one is worked on.
+template <class T, class W, int E, int PPL, int G, int BT, int OCC, bool AHEAD>
+__global__ __launch_bounds__(BT, OCC) void norm_grad_kernel(NormBwd a)
 {
     using A = acc_of<T>;
     constexpr int NG = BT / G;
-    __shared__ A lds[2][BT / 64][2];
+    __shared__ SumPart<2, A> lds[2][BT / 16];
     extern __shared__ __attribute__((aligned(16))) char cols_raw[]; // NG > 1: [2][n] sums of the block's groups
-    const int li = threadIdx.x % G, gi = threadIdx.x / G;
+    const int li = NG > 1 ? threadIdx.x % G : threadIdx.x, gi = NG > 1 ? threadIdx.x / G : 0; // (one row a block: uniform)
     const int64_t n = a.n, step = (int64_t)gridDim.x * NG;
     const PackAt<E, G> last(n, li, PPL - 1);
     A w[PPL][E], dw[PPL][E], db[PPL][E];
@@ -175,44 +219,65 @@ template <class T, class W, int E, int PPL, int G, int BT> __global__ __launch_b
             dw[j][e] = db[j][e] = 0;
         }
     }
-    int slot = 0;
-    for (int64_t row = (int64_t)blockIdx.x * NG + gi; row < a.map.rows; row += step, slot ^= 1) {
+    struct Row {
+        pack<T, E> x[PPL], dy[PPL];
+        A mean, rstd;
+        T *dx;
+    };
+    auto fetch = [&](int64_t row, Row &r) {
         const T *dy = (const T *)a.dy + a.map.template off<0>(row), *x = (const T *)a.x + a.map.template off<1>(row);
-        const A mean = ((const A *)a.mean)[a.map.template off<3>(row)], rstd = ((const A *)a.rstd)[a.map.template off<4>(row)];
-        A g[PPL][E], h[PPL][E];
 #pragma unroll
         for (int j = 0; j < PPL; ++j) {
             const PackAt<E, G> at(n, li, j);
-            load_vals<E, true>(dy + at.base, g[j]);
-            load_vals<E, true>(x + at.base, h[j]);
+            r.dy[j] = load_pack<T, E>(dy + at.base);
+            r.x[j] = load_pack<T, E>(x + at.base);
         }
+        r.dx = (T *)a.dx + a.map.template off<2>(row);
+        r.mean = ((const A *)a.mean)[a.map.template off<3>(row)];
+        r.rstd = ((const A *)a.rstd)[a.map.template off<4>(row)];
+    };
+    const A inv_n = A(1) / (A)n;
+    const bool tail = __builtin_amdgcn_ballot_w64(last.skip != 0) != 0; // some lane of the wave
+    int slot = 0;
+    int64_t row = (int64_t)blockIdx.x * NG + gi;
+    Row r;
+    if (AHEAD && row < a.map.rows) fetch(row, r);
+    for (; row < a.map.rows; row += step, slot ^= 1) {
+        // (loads and stores are never conditional: the wait for the next row's loads then leaves this row's stores in flight)
+        Row next;
+        if constexpr (!AHEAD) fetch(row, r);
+        else fetch(row + step < a.map.rows ? row + step : row, next);
+        auto centred = [&](T x) { return ((A)x - r.mean) * r.rstd; };
         A s[2] = {0, 0};
+        pack<T, E> dy_last = r.dy[PPL - 1];
+        if (tail) // elements that another lane owns add nothing
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < last.skip) dy_last.v[e] = (T)0;
 #pragma unroll
         for (int j = 0; j < PPL; ++j)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const bool mine = j < PPL - 1 || e >= last.skip;
-                h[j][e] = (h[j][e] - mean) * rstd;
-                const A d = mine ? g[j][e] : A(0);
-                dw[j][e] += d * h[j][e];
+                const A h = centred(r.x[j].v[e]), d = (A)(j < PPL - 1 ? r.dy[j] : dy_last).v[e], g = d * w[j][e];
+                dw[j][e] = row_fma(d, h, dw[j][e]);
                 db[j][e] += d;
-                g[j][e] *= w[j][e];
-                const A gw = mine ? g[j][e] : A(0);
-                s[0] += gw;
-                s[1] += gw * h[j][e];
+                s[0] += g;
+                s[1] = row_fma(g, h, s[1]);
             }
         row_sums<G, BT>(s, lds, slot);
-        const A c1 = s[0] / (A)n, c2 = s[1] / (A)n;
-        T *dx = (T *)a.dx + a.map.template off<2>(row);
+        const A c1 = s[0] * inv_n, c2 = s[1] * inv_n;
 #pragma unroll
         for (int j = 0; j < PPL; ++j) {
             const PackAt<E, G> at(n, li, j);
-            if (at.skip >= E) continue;
             A o[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = (g[j][e] - c1 - h[j][e] * c2) * rstd;
-            store_vals<E, true>(dx + at.base, o);
+            for (int e = 0; e < E; ++e) {
+                const A g = (A)r.dy[j].v[e] * w[j][e];
+                o[e] = row_fma(-centred(r.x[j].v[e]), c2, g - c1) * r.rstd;
+            }
+            store_vals<E, true>(r.dx + at.base, o); // (a last pack's first elements are also the lane's before: the same values)
         }
+        if constexpr (AHEAD) r = next;
     }
     if (!a.part) return;
     A *part = (A *)a.part + (int64_t)blockIdx.x * 2 * n;
@@ -254,7 +319,7 @@ template <class T, class W, int E, int PPL, int G, int BT> __global__ __launch_b
 template <class T, class W, int BT> __global__ __launch_bounds__(BT) void norm_grad_long_kernel(NormBwd a)
 {
     using A = acc_of<T>;
-    __shared__ A lds[2][BT / 64][2];
+    __shared__ SumPart<2, A> lds[2][BT / 16];
     const int64_t n = a.n;
     A *part = a.part ? (A *)a.part + (int64_t)blockIdx.x * 2 * n : nullptr;
     int slot = 0;
@@ -282,20 +347,27 @@ template <class T, class W, int BT> __global__ __launch_bounds__(BT) void norm_g
     }
 }
 
-// dw and db: the blocks' sums added up in block order.  64 columns by 16 threads that each take every 16th block.
-constexpr int FOLD_COLS = 64, FOLD_ROWS = 16;
+// dw and db: the blocks' sums added up in a fixed order.  32 columns by 32 threads that each take every 32nd block, eight
+// loads at a time.
+constexpr int FOLD_COLS = 32, FOLD_ROWS = 16, FOLD_U = 16;
 template <class W, class A>
 __global__ __launch_bounds__(FOLD_COLS *FOLD_ROWS) void norm_grad_fold_kernel(const A *part, int64_t blocks, int64_t n, W *dw, W *db)
 {
-    __shared__ A lds[FOLD_ROWS][FOLD_COLS];
+    __shared__ A lds[FOLD_ROWS][FOLD_COLS + 1];
     const int c = threadIdx.x % FOLD_COLS, r = threadIdx.x / FOLD_COLS;
     const int64_t col = (int64_t)blockIdx.x * FOLD_COLS + c; // over the 2 n columns of dw and db
     A s = 0;
     if (col < 2 * n)
-        for (int64_t k = r; k < blocks; k += FOLD_ROWS) s += part[k * 2 * n + col];
+        for (int64_t k = r; k < blocks; k += FOLD_ROWS * FOLD_U) {
+            A v[FOLD_U];
+#pragma unroll
+            for (int u = 0; u < FOLD_U; ++u) v[u] = k + u * FOLD_ROWS < blocks ? part[(k + u * FOLD_ROWS) * 2 * n + col] : A(0);
+#pragma unroll
+            for (int u = 0; u < FOLD_U; ++u) s += v[u];
+        }
     lds[r][c] = s;
     __syncthreads();
-    if (r == 0 && col < 2 * n) {
+    if (threadIdx.x < FOLD_COLS && col < 2 * n) {
 #pragma unroll
         for (int k = 1; k < FOLD_ROWS; ++k) s += lds[k][c];
         if (col < n) dw[col] = (W)s;
@@ -304,12 +376,12 @@ __global__ __launch_bounds__(FOLD_COLS *FOLD_ROWS) void norm_grad_fold_kernel(co
 }
 
 // ---- dispatch --------------------------------------------------------------------------------------------------------
-// Lanes and packs per lane for rows of n elements: the fewest lanes that hold the row, a wave up to 4 packs per lane, then
+// Lanes and packs per lane for rows of n elements: the fewest lanes that hold the row, a wave up to 2 packs per lane, then
 // blocks of 256, 512 and 1024 threads.  g = 0: the row does not fit.
 struct NormShape {
     int e, g, ppl, bt;
 };
-template <class T> NormShape norm_shape(int64_t n, int max_block_ppl)
+template <class T> NormShape norm_shape(int64_t n)
 {
     constexpr int E = 16 / (int)sizeof(T);
     if (n < E) return {1, 8, 1, 256};
@@ -317,12 +389,22 @@ template <class T> NormShape norm_shape(int64_t n, int max_block_ppl)
     if (p <= 8) return {E, 8, 1, 256};
     if (p <= 16) return {E, 16, 1, 256};
     if (p <= 32) return {E, 32, 1, 256};
-    if (p <= 256) return {E, 64, (int)((p + 63) / 64), 256};
+    if (p <= 128) return {E, 64, (int)((p + 63) / 64), 256};
+    if (p <= 256) return {E, 256, 1, 256};
     for (int bt : {256, 512, 1024}) {
         const int64_t ppl = (p + bt - 1) / bt;
-        if (ppl <= (bt == 1024 ? max_block_ppl : 4)) return {E, bt, (int)ppl, bt};
+        if (ppl <= (bt == 1024 ? 8 : 4)) return {E, bt, (int)ppl, bt};
     }
     return {0, 0, 0, 1024};
+}
+
+// Blocks per CU: as many as keep about 22 KiB of the next rows on their way.  (More streams worse, fewer leaves latency
+// uncovered: 16384 x 4096 float16, 8 KiB a block, 2 / 3 / 4 / 5 / 8 blocks a CU: 50.7 / 46.4 / 47.0 / 49.3 / 51.8 us;
+// 20011 x 1001 float32, 4 KiB a block: 44.0 / 34.8 / 30.0 / 29.5 / 31.4.)
+inline int norm_per_cu(const NormShape &s)
+{
+    const int bytes = s.bt * s.ppl * 16;
+    return std::max(1, std::min(5, (22 * 1024 + bytes / 2) / std::max(bytes, 1)));
 }
 
 // calls f(integral constants E, PPL, G, BT) for a shape of norm_shape
@@ -340,8 +422,7 @@ template <int E, class F> bool norm_dispatch(const NormShape &s, F &&f)
     DPX_NORM_CASE(E, 1, 32, 256)
     DPX_NORM_CASE(E, 1, 64, 256)
     DPX_NORM_CASE(E, 2, 64, 256)
-    DPX_NORM_CASE(E, 3, 64, 256)
-    DPX_NORM_CASE(E, 4, 64, 256)
+    DPX_NORM_CASE(E, 1, 256, 256)
     DPX_NORM_CASE(E, 2, 256, 256)
     DPX_NORM_CASE(E, 3, 256, 256)
     DPX_NORM_CASE(E, 4, 256, 256)
@@ -366,9 +447,8 @@ constexpr int64_t MAX_GRID = 0x7fffffff;
 template <class T, class W> int norm_fwd_launch(const NormFwd &a, hipStream_t s)
 {
     constexpr int E = 16 / (int)sizeof(T);
-    const NormShape sh = norm_shape<T>(a.n, 8);
-    const int64_t per = sh.g ? sh.bt / sh.g : 1, grid = (a.map.rows + per - 1) / per;
-    if (grid > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, "layer_norm: too many rows for one launch");
+    const NormShape sh = norm_shape<T>(a.n);
+    const int64_t per = sh.g ? sh.bt / sh.g : 1, grid = std::min<int64_t>((a.map.rows + per - 1) / per, (int64_t)device_cus() * norm_per_cu(sh));
     auto run = [&](auto e, auto ppl, auto g, auto bt) {
         hipLaunchKernelGGL((norm_fwd_kernel<T, W, decltype(e)::value, decltype(ppl)::value, decltype(g)::value, decltype(bt)::value>),
                            dim3((unsigned)grid), dim3(bt), 0, s, a);
@@ -379,13 +459,67 @@ template <class T, class W> int norm_fwd_launch(const NormFwd &a, hipStream_t s)
     return rc == hipSuccess ? DPX_OK : fail_hip(rc, "layer_norm launch");
 }
 
-// blocks of the backward kernel
+// Shapes of the backward kernel: like norm_shape, with fewer packs per lane (a pack of E elements costs 2 E registers for the
+// column sums, E for the weights and 16 for the row and the next one), and as many blocks as stay resident.
+struct GradShape {
+    int e, g, ppl, bt, per_cu;
+};
+template <class T> GradShape grad_shape(int64_t n)
+{
+    constexpr int E = 16 / (int)sizeof(T);
+    if (n < E) return {1, 8, 1, 256, 4};
+    const int64_t p = (n + E - 1) / E;
+    if (p <= 8) return {E, 8, 1, 256, 4};
+    if (p <= 16) return {E, 16, 1, 256, 4};
+    if (p <= 32) return {E, 32, 1, 256, 4};
+    if (p <= (E == 8 ? 64 : 128)) return {E, 64, (int)((p + 63) / 64), 256, 4};
+    if (p <= 256) return {E, 256, 1, 256, 4};
+    if (p <= 512) return {E, 512, 1, 512, 2};
+    if (p <= 1024) return E == 4 ? GradShape{E, 512, 2, 512, 2} : GradShape{E, 1024, 1, 1024, 1};
+    const int64_t ppl = (p + 511) / 512;
+    if (ppl <= (E == 8 ? 4 : 8)) return {E, 512, (int)ppl, 512, 1};
+    return {0, 0, 0, 1024, 1};
+}
+template <int E, class F> bool grad_dispatch(const GradShape &s, F &&f)
+{
+#define DPX_GRAD_CASE(E_, P_, G_, B_, O_, A_)                                                                                  \
+    if (s.e == (E_) && s.ppl == (P_) && s.g == (G_)) {                                                                         \
+        f(std::integral_constant<int, (E_)>{}, std::integral_constant<int, (P_)>{}, std::integral_constant<int, (G_)>{},       \
+          std::integral_constant<int, (B_)>{}, std::integral_constant<int, (O_)>{}, std::integral_constant<bool, (A_)>{});     \
+        return true;                                                                                                           \
+    }
+    DPX_GRAD_CASE(1, 1, 8, 256, 4, true)
+    DPX_GRAD_CASE(E, 1, 8, 256, 4, true)
+    DPX_GRAD_CASE(E, 1, 16, 256, 4, true)
+    DPX_GRAD_CASE(E, 1, 32, 256, 4, true)
+    DPX_GRAD_CASE(E, 1, 64, 256, 4, true)
+    if constexpr (E < 8) DPX_GRAD_CASE(E, 2, 64, 256, 4, true)
+    DPX_GRAD_CASE(E, 1, 256, 256, 4, true)
+    DPX_GRAD_CASE(E, 1, 512, 512, 4, true)
+    if constexpr (E == 4) {
+        DPX_GRAD_CASE(E, 2, 512, 512, 4, true)
+    }
+    else {
+        DPX_GRAD_CASE(E, 1, 1024, 1024, 4, true)
+    }
+    DPX_GRAD_CASE(E, 3, 512, 512, 2, E != 8)
+    DPX_GRAD_CASE(E, 4, 512, 512, 2, E != 8)
+    if constexpr (E < 8) {
+        DPX_GRAD_CASE(E, 5, 512, 512, 2, E == 4)
+        DPX_GRAD_CASE(E, 6, 512, 512, 2, false)
+        DPX_GRAD_CASE(E, 7, 512, 512, 2, false)
+        DPX_GRAD_CASE(E, 8, 512, 512, 2, false)
+    }
+#undef DPX_GRAD_CASE
+    return false;
+}
 template <class T> int64_t norm_grad_blocks(int64_t rows, int64_t n)
 {
-    const NormShape sh = norm_shape<T>(n, 0);
-    const int64_t per = sh.g ? sh.bt / sh.g : 1, need = (rows + per - 1) / per;
-    const int64_t want = (int64_t)device_cus() * (sh.bt <= 256 ? 4 : sh.bt == 512 ? 2 : 1);
-    return std::min(need, want);
+    const GradShape sh = grad_shape<T>(n);
+    const int64_t per = sh.g ? sh.bt / sh.g : 1, need = (rows + per - 1) / per, slots = (int64_t)device_cus() * sh.per_cu;
+    if (need <= slots) return need;
+    const int64_t turns = (need + slots - 1) / slots; // the fewest blocks that need no more turns: they end together
+    return (need + turns - 1) / turns;
 }
 
 template <class T, class W> int norm_grad_launch(NormBwd &a, void *dw, void *db, hipStream_t s)
@@ -394,13 +528,14 @@ template <class T, class W> int norm_grad_launch(NormBwd &a, void *dw, void *db,
     constexpr int E = 16 / (int)sizeof(T);
     const int64_t blocks = norm_grad_blocks<T>(a.map.rows, a.n);
     if (blocks > 0) {
-        const NormShape sh = norm_shape<T>(a.n, 0);
-        auto run = [&](auto e, auto ppl, auto g, auto bt) {
+        const GradShape sh = grad_shape<T>(a.n);
+        auto run = [&](auto e, auto ppl, auto g, auto bt, auto occ, auto ahead) {
             const size_t lds = (a.part && sh.g < sh.bt) ? (size_t)(2 * a.n) * sizeof(A) : 0;
-            hipLaunchKernelGGL((norm_grad_kernel<T, W, decltype(e)::value, decltype(ppl)::value, decltype(g)::value, decltype(bt)::value>),
+            hipLaunchKernelGGL((norm_grad_kernel<T, W, decltype(e)::value, decltype(ppl)::value, decltype(g)::value, decltype(bt)::value,
+                                                 decltype(occ)::value, decltype(ahead)::value>),
                                dim3((unsigned)blocks), dim3(bt), lds, s, a);
         };
-        if (!norm_dispatch<E>(sh, run))
+        if (!grad_dispatch<E>(sh, run))
             hipLaunchKernelGGL((norm_grad_long_kernel<T, W, 1024>), dim3((unsigned)blocks), dim3(1024), 0, s, a);
     }
     if (dw) {

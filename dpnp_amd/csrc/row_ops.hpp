@@ -19,10 +19,11 @@ template <int NOPS> struct RowMap {
     {
         if (nd <= 1) return r * st1[K];
         int64_t o = 0;
+        uint32_t q = (uint32_t)r; // (rows < 2^31, checked on the host: a 64-bit division takes as many registers as a row)
         for (int d = nd - 1; d >= 0; --d) {
-            const int64_t q = r / shape[d];
-            o += (r - q * shape[d]) * st[K][d];
-            r = q;
+            const uint32_t e = (uint32_t)shape[d], t = q / e;
+            o += (int64_t)(q - t * e) * st[K][d];
+            q = t;
         }
         return o;
     }
@@ -83,6 +84,7 @@ template <class F> int row_entry(F &&f)
 }
 
 // ---- device: sums over the lanes that share a row ----------------------------------------------------------------------
+// (only for permutations inside a row of 16 lanes: every lane has a source)
 template <int CTRL, class A> DPX_D A dpp_get(A v)
 {
     constexpr int W = sizeof(A) / 4;
@@ -92,7 +94,7 @@ template <int CTRL, class A> DPX_D A dpp_get(A v)
     } u;
     u.a = v;
 #pragma unroll
-    for (int i = 0; i < W; ++i) u.w[i] = __builtin_amdgcn_update_dpp(u.w[i], u.w[i], CTRL, 0xf, 0xf, false);
+    for (int i = 0; i < W; ++i) u.w[i] = __builtin_amdgcn_mov_dpp(u.w[i], CTRL, 0xf, 0xf, true);
     return u.a;
 }
 template <class A> DPX_D A lane_get(A v, int lane)
