@@ -164,7 +164,7 @@ SIGNATURES = {
     "dpx_layer_norm": (_i, [_VP, _VP, _VP, _d, _VP, _VP, _VP, _vp]),
     "dpx_layer_norm_grad_workspace": (_i64, [_VP]),
     "dpx_layer_norm_grad": (_i, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _vp, ctypes.c_size_t, _vp]),
-    "dpx_distill_topk_workspace": (_i64, [_VP]),
+    "dpx_distill_topk_workspace": (_i64, [_VP, _VP]),
     "dpx_distill_topk": (_i, [_VP, _VP, _VP, _d, _VP, _vp, ctypes.c_size_t, _vp]),
     "dpx_distill_topk_grad": (_i, [_VP, _VP, _VP, _VP, _d, _VP, _VP, _vp, ctypes.c_size_t, _vp]),
     "dpx_process_logits": (_i, [_VP, ctypes.POINTER(LogitsArgs), _VP, _vp]),

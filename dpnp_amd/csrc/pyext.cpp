@@ -438,7 +438,7 @@ void distill_topk(py::handle logits, py::handle teacher, py::handle tokens, py::
 {
     dpx_array_view *vz = view_arg(logits, "logits"), *vt = view_arg(teacher, "teacher_logits"),
                    *vi = view_arg(tokens, "teacher_tokens"), *vl = view_arg(loss, "loss");
-    const Workspace ws(dpx_distill_topk_workspace(vz));
+    const Workspace ws(dpx_distill_topk_workspace(vz, vt));
     void *s = stream_of(py::none());
     const int rc = dlogits.is_none()
                        ? dpx_distill_topk(vz, vt, vi, temperature, vl, ws.data, ws.bytes, s)

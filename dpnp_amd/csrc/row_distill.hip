@@ -5,10 +5,15 @@
 //   loss = T^2 sum_k p_k (log p_k - log q[i_k])            (a term with p_k = 0 is 0; no entries: the loss is 0)
 //   d loss / d z[v] = T (q[v] P - sum over k with i_k = v of p_k),   P = sum_k p_k: 1, or 0 where no entry is there
 //
-// The vocabulary is what costs: the loss reads V logits, the gradient reads and writes V.  One pass keeps a running
-// maximum m and s = sum exp((z - m) / T) per thread; rows are split over blocks and joined through partials (m, s) in the
-// caller's workspace.  Exponentials are taken of z - m (not of z scaled and shifted in one step, whose rounding grows with
-// the logits' common offset).  Statistics and sums are float32 (float64 for float64 logits).
+// The vocabulary is what costs: the loss reads V logits, the gradient reads and writes V.  Exponentials are taken to base 2:
+// e_v = 2^(z_v c - M) with c = log2(e) / T, M = c max(z) rounded, as one fused multiply-add and one exponential instruction.
+// M's rounding multiplies every e_v of the row by the same factor, which the sum s = sum e_v takes out again (log q_v =
+// (z_v c - M) ln 2 - ln s, with the same M), so a common offset of the logits costs no accuracy.  Statistics and sums are
+// float32 (float64 for float64 logits).
+//
+// Many rows: a block owns a row.  Its logits are read once, HELD packs per thread stay in registers between the sum and the
+// gradient, what does not fit is read again while it is still in a cache.  Few rows: a row is split over blocks that leave
+// (M, s) in the caller's workspace, and a second launch joins them.
 #include "row_ops.hpp"
 #include <algorithm>
 
@@ -19,240 +24,343 @@ struct Distill {
     RowMap<6> map; // logits, teacher, tokens, weights, loss, dlogits
     const void *z, *t, *tok, *wt;
     void *loss, *dz;
-    void *part; // [rows][splits] pairs (m, s)
+    void *part; // split rows: [rows][splits] pairs (M, s), then [rows][3 k + 2] values of the teacher's side
     int64_t v, chunk;
     int32_t k, tok64, splits;
     double temp;
 };
 
-// e^((x - m) / T) as 2^((x - m) c), c = log2(e) / T
 DPX_D float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 DPX_D double pow2(double x) { return ::exp2(x); }
 DPX_D float ln(float x) { return ::logf(x); }
 DPX_D double ln(double x) { return ::log(x); }
+DPX_D float fma1(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+DPX_D double fma1(double a, double b, double c) { return __builtin_fma(a, b, c); }
 template <class A> DPX_D A neg_inf() { return -(A)__builtin_inff(); }
+template <class A> DPX_D A scale_of(const Distill &a) { return (A)(1.4426950408889634074 / a.temp); }
 
-// running maximum and sum of exponentials.  While m is -inf (nothing but -inf so far) the exponentials are taken relative
-// to 0, which leaves the sum at 0 and lets a NaN through.
+// Largest scaled logit M and sum of 2^(z c - M).  While M is -inf (nothing but -inf so far) the exponentials are taken relative
+// to 0, which leaves the sum at 0 and lets a NaN through; the maximum itself passes NaN over.
 template <class A> struct Soft {
     A m, s;
 };
 template <class A> DPX_D A anchor(A m) { return m == neg_inf<A>() ? A(0) : m; }
-template <class A> DPX_D Soft<A> soft_join(Soft<A> a, Soft<A> b, A c)
+template <class A> DPX_D Soft<A> soft_join(Soft<A> a, Soft<A> b)
 {
     const A m = MaxOp{}(a.m, b.m), z = anchor(m);
-    return {m, a.s * pow2((a.m - z) * c) + b.s * pow2((b.m - z) * c)};
+    return {m, a.s * pow2(a.m - z) + b.s * pow2(b.m - z)};
 }
-
-// over a block: by DPP inside the waves, then through LDS; the result in every thread
-template <int BT, class A> DPX_D Soft<A> soft_block(Soft<A> v, A c, A (*lds)[2])
+// over G lanes, the result in all of them
+template <int G, class A> DPX_D Soft<A> soft_lanes(Soft<A> v)
 {
-    const A m = lanes_fold<64>(v.m, MaxOp{}), z = anchor(m);
-    v.s = lanes_fold<64>(v.s * pow2((v.m - z) * c), SumOp{});
-    v.m = m;
-    if constexpr (BT > 64) {
-        const int wave = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) {
-            lds[wave][0] = v.m;
-            lds[wave][1] = v.s;
-        }
-        __syncthreads();
-        A mm = lds[0][0];
-#pragma unroll
-        for (int k = 1; k < BT / 64; ++k) mm = MaxOp{}(mm, lds[k][0]);
-        const A zz = anchor(mm);
-        A s = 0;
-#pragma unroll
-        for (int k = 0; k < BT / 64; ++k) s += lds[k][1] * pow2((lds[k][0] - zz) * c);
-        v.m = mm;
-        v.s = s;
-    }
-    return v;
+    const A m = lanes_fold<G>(v.m, MaxOp{});
+    return {m, lanes_fold<G>(v.s * pow2(v.m - anchor(m)), SumOp{})};
+}
+// over a block of up to 1024 threads, in two halves around a barrier of the caller's
+template <class A> DPX_D void soft_leave(Soft<A> v, Soft<A> *lds)
+{
+    v = soft_lanes<64>(v);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+}
+template <int BT, class A> DPX_D Soft<A> soft_collect(const Soft<A> *lds)
+{
+    constexpr int NW = BT / 64;
+    static_assert(NW == 4 || NW == 8 || NW == 16);
+    // every row of 16 lanes reads all waves' values (more than once where there are fewer: the duplicates are left out)
+    const int lane = threadIdx.x & 15;
+    Soft<A> v = lds[lane & (NW - 1)];
+    if (lane >= NW) v.s = 0;
+    return soft_lanes<16>(v);
 }
 
-// the (m, s) of elements [begin, end) of a row, over a block
-template <class T, int BT> DPX_D Soft<acc_of<T>> soft_scan(const T *z, int64_t begin, int64_t end, acc_of<T> c)
+template <class T, int E> DPX_D acc_of<T> pack_max(const pack<T, E> &v)
 {
     using A = acc_of<T>;
-    constexpr int E = 16 / (int)sizeof(T), U = 4;
-    Soft<A> r{neg_inf<A>(), 0};
-    auto take = [&](const A(&x)[E]) {
-        A m = r.m;
+    T m = v.v[0];
 #pragma unroll
-        for (int e = 0; e < E; ++e) m = MaxOp{}(m, x[e]);
-        const A a = anchor(m);
-        A s = r.s * pow2((r.m - a) * c);
-#pragma unroll
-        for (int e = 0; e < E; ++e) s += pow2((x[e] - a) * c);
-        r.m = m;
-        r.s = s;
-    };
-    int64_t i = begin + (int64_t)threadIdx.x * E;
-    for (; i + (int64_t)(U - 1) * BT * E + E <= end; i += (int64_t)U * BT * E) {
-        A x[U][E];
-#pragma unroll
-        for (int u = 0; u < U; ++u) load_vals<E, false>(z + i + (int64_t)u * BT * E, x[u]);
-#pragma unroll
-        for (int u = 0; u < U; ++u) take(x[u]);
-    }
-    for (; i + E <= end; i += (int64_t)BT * E) {
-        A x[E];
-        load_vals<E, false>(z + i, x);
-        take(x);
-    }
-    if (i < end) { // the range's last, partial pack
-        A x[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = i + e < end ? (A)z[i + e] : neg_inf<A>();
-        take(x);
-    }
-    return r;
+    for (int e = 1; e < E; ++e) m = __builtin_elementwise_max(m, v.v[e]);
+    return (A)m;
 }
-
-DPX_D int64_t token_at(const void *tok, int is64, int64_t i)
+template <class T, int E> DPX_D pack<T, E> pack_max2(pack<T, E> a, const pack<T, E> &b)
 {
-    return is64 ? ((const int64_t *)tok)[i] : (int64_t)((const int32_t *)tok)[i];
+#pragma unroll
+    for (int e = 0; e < E; ++e) a.v[e] = __builtin_elementwise_max(a.v[e], b.v[e]);
+    return a;
+}
+// U packs joined into a running (M, s): one rescaling for all of them
+template <class T, int E, int U, class A> DPX_D void soft_take(Soft<A> &r, const pack<T, E> *x, A c)
+{
+    pack<T, E> top = x[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u) top = pack_max2(top, x[u]);
+    const A m = MaxOp{}(r.m, pack_max(top) * c), z = anchor(m);
+    A s[4] = {r.s * pow2(r.m - z), 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[(u * E + e) & 3] += pow2(fma1((A)x[u].v[e], c, -z));
+    r.m = m;
+    r.s = (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-// The teacher's distribution of a row: p[k] (0 where absent) and token[k] (-1 where absent) in LDS, by a block; returns
-// sum(p): 1, 0 with no entry that counts, or NaN.  ends with a barrier.  log_norm: log p_k = (t_k - m) / T - log_norm.
-template <class A> struct Teacher {
-    A mass, m, log_norm;
+// A run of n elements, as packs and fewer than E elements behind them, which the block's first threads take one each.
+template <class T, int E> struct Run {
+    const T *z;
+    int packs, rest;
+    DPX_D Run(const T *z_, int n) : z(z_), packs(n / E), rest(n % E) {}
+    template <bool NT> DPX_D pack<T, E> load(int p) const // -inf beyond the run
+    {
+        pack<T, E> x;
+        if (p < packs) return load_pack<T, E, NT>(z + p * E);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x.v[e] = (T)(-__builtin_inff());
+        return x;
+    }
+    DPX_D T load_rest(int i) const { return i < rest ? z[packs * E + i] : (T)(-__builtin_inff()); }
+    // f(z) of every element of pack p
+    template <class F> DPX_D void store(T *dz, int p, const pack<T, E> &x, F f) const
+    {
+        acc_of<T> o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = f(x.v[e]);
+        if (p < packs) store_vals<E, true>(dz + p * E, o);
+    }
+    template <class F> DPX_D void store_rest(T *dz, int i, T x, F f) const
+    {
+        if (i < rest) dz[packs * E + i] = (T)f(x);
+    }
 };
-template <class TT, int BT, class A>
-DPX_D Teacher<A> teacher_row(const Distill &a, int64_t row, A inv_t, A c, A *p, int32_t *token, A (*lds)[2])
+template <class T, class A> DPX_D Soft<A> soft_one(Soft<A> r, T x, A c) // one element more
 {
+    const A m = MaxOp{}(r.m, (A)x * c), z = anchor(m);
+    return {m, r.s * pow2(r.m - z) + pow2(fma1((A)x, c, -z))};
+}
+
+// ---- the teacher's side of a row, by one wave -----------------------------------------------------------------------------
+// p[k] (0 where absent), the student's logit zk[k] at the entry's token and the token itself (-1 where absent); in `sum` the
+// mass sum(p) (1, 0 with no entry that counts, or NaN) and sum p ln p.
+template <class A> struct TeacherSum {
+    A mass, plogp;
+};
+template <class T, class TT, class A>
+DPX_D TeacherSum<A> teacher_wave(const Distill &a, int64_t row, A c, A *p, A *zk, int32_t *token)
+{
+    const int lane = threadIdx.x & 63;
+    const T *z = (const T *)a.z + a.map.template off<0>(row);
     const TT *t = (const TT *)a.t + a.map.template off<1>(row);
     const int64_t to = a.map.template off<2>(row);
     Soft<A> s{neg_inf<A>(), 0};
-    for (int k = threadIdx.x; k < a.k; k += BT) {
-        const int64_t i = token_at(a.tok, a.tok64, to + k);
+    for (int k = lane; k < a.k; k += 64) {
+        const int64_t i = a.tok64 ? ((const int64_t *)a.tok)[to + k] : (int64_t)((const int32_t *)a.tok)[to + k];
         const bool there = i >= 0 && i < a.v;
-        token[k] = there ? (int32_t)i : -1;
         const A x = there ? (A)t[k] : neg_inf<A>();
+        token[k] = there ? (int32_t)i : -1;
+        zk[k] = there ? (A)z[i] : A(0);
         p[k] = x;
-        s = soft_join(s, Soft<A>{x, there ? pow2((x - anchor(x)) * c) : A(0)}, c);
+        const A m = MaxOp{}(s.m, x * c), anc = anchor(m);
+        s.s = s.s * pow2(s.m - anc) + pow2(fma1(x, c, -anc));
+        s.m = m;
     }
-    s = soft_block<BT>(s, c, lds);
+    s = soft_lanes<64>(s);
     const bool none = s.m == neg_inf<A>() && s.s == 0;
-    const A inv = none ? A(0) : A(1) / s.s;
-    for (int k = threadIdx.x; k < a.k; k += BT) p[k] = none ? A(0) : pow2((p[k] - anchor(s.m)) * c) * inv;
-    __syncthreads();
-    return {none ? A(0) : s.s * inv, anchor(s.m), ln(s.s)};
+    const A inv = none ? A(0) : A(1) / s.s, m = anchor(s.m), lns = ln(s.s);
+    A plogp = 0;
+    for (int k = lane; k < a.k; k += 64) {
+        const A e = fma1(p[k], c, -m), pk = none ? A(0) : pow2(e) * inv;
+        p[k] = pk;
+        if (pk != 0) plogp += pk * (e * (A)0.69314718055994530942 - lns);
+    }
+    return {none ? A(0) : s.s * inv, lanes_fold<64>(plogp, SumOp{})};
 }
-
-// loss of a row, in thread 0 (a block; p and token from teacher_row)
-template <class T, class TT, int BT, class A>
-DPX_D A row_loss(const Distill &a, int64_t row, const T *z, Soft<A> q, const Teacher<A> &te, A inv_t, const A *p, const int32_t *token,
-                 A (*lds)[2])
+// loss of the row from the student's (M, s): by one wave
+template <class A> DPX_D A loss_wave(const Distill &a, Soft<A> q, TeacherSum<A> te, A c, const A *p, const A *zk)
 {
-    const TT *t = (const TT *)a.t + a.map.template off<1>(row);
-    const A lq = ln(q.s);
+    const A lns = ln(q.s);
     A sum = 0;
-    for (int k = threadIdx.x; k < a.k; k += BT) {
-        const A pk = p[k];
-        if (token[k] < 0 || pk == 0) continue;
-        const A logp = ((A)t[k] - te.m) * inv_t - te.log_norm;
-        const A logq = ((A)z[token[k]] - q.m) * inv_t - lq;
-        sum += pk * (logp - logq);
-    }
+    for (int k = threadIdx.x & 63; k < a.k; k += 64)
+        if (p[k] != 0) sum += p[k] * (fma1(zk[k], c, -q.m) * (A)0.69314718055994530942 - lns);
     sum = lanes_fold<64>(sum, SumOp{});
-    if constexpr (BT > 64) {
-        __syncthreads(); // lds was read by the sum before
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6][0] = sum;
-        __syncthreads();
-        sum = 0;
-#pragma unroll
-        for (int k = 0; k < BT / 64; ++k) sum += lds[k][0];
-    }
-    // a NaN among the teacher's logits makes every p NaN; a row without entries gives 0
-    return te.mass == 0 ? A(0) : (A)(a.temp * a.temp) * sum;
+    return te.mass == 0 ? A(0) : (A)(a.temp * a.temp) * (te.plogp - sum);
+}
+// all the weight that entry k's token gets, its own and that of other entries with the same token, in their order
+template <class A> DPX_D A same_token(const Distill &a, const A *p, const int32_t *token, int k)
+{
+    const int32_t i = token[k];
+    A sum = 0;
+    for (int j = 0; j < a.k; ++j) sum += token[j] == i ? p[j] : A(0);
+    return sum;
 }
 
-constexpr int DST_BLOCK = 256;
-
-// partials of every row: block (row, split)
-template <class T> __global__ __launch_bounds__(DST_BLOCK) void distill_stats_kernel(Distill a)
+// ---- many rows: a block owns a row ----------------------------------------------------------------------------------------
+// The gradient is stored densely first, a barrier, then the values at the teacher's tokens over it (their logits were read at
+// the start: dz may be z).  A row of weight 0, and one without entries, gets zeros whatever its logits are.
+template <class T, class TT, int BT, int HELD, bool GRAD>
+__global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_kernel(Distill a)
 {
     using A = acc_of<T>;
-    __shared__ A lds[DST_BLOCK / 64][2];
-    const int64_t row = blockIdx.x / (uint32_t)a.splits;
-    const int split = (int)(blockIdx.x - (uint32_t)row * (uint32_t)a.splits);
-    const T *z = (const T *)a.z + a.map.template off<0>(row);
-    const int64_t begin = split * a.chunk, end = begin + a.chunk < a.v ? begin + a.chunk : a.v;
-    const A c = (A)(1.4426950408889634074 / a.temp);
-    const Soft<A> r = soft_block<DST_BLOCK>(soft_scan<T, DST_BLOCK>(z, begin, end, c), c, lds);
-    if (threadIdx.x == 0) ((Soft<A> *)a.part)[blockIdx.x] = r;
+    constexpr int E = 16 / (int)sizeof(T), U = 4;
+    static_assert(HELD % U == 0);
+    extern __shared__ __attribute__((aligned(16))) char raw[];
+    __shared__ Soft<A> waves[BT / 64];
+    __shared__ TeacherSum<A> teacher;
+    A *p = (A *)raw, *zk = p + a.k;
+    int32_t *token = (int32_t *)(zk + a.k);
+    const int64_t row = blockIdx.x;
+    const int tid = (int)threadIdx.x;
+    const Run<T, E> run((const T *)a.z + a.map.template off<0>(row), (int)a.v);
+    T *dz = GRAD ? (T *)a.dz + a.map.template off<5>(row) : nullptr;
+    const A c = scale_of<A>(a);
+    pack<T, E> held[HELD ? HELD : 1];
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) held[j] = run.template load<true>(j * BT + tid);
+    const T rest = run.load_rest(tid);
+    if (tid < 64) {
+        const TeacherSum<A> te = teacher_wave<T, TT, A>(a, row, c, p, zk, token);
+        if (tid == 0) teacher = te;
+    }
+    const A w = GRAD ? (a.wt ? ((const A *)a.wt)[a.map.template off<3>(row)] : A(1)) : A(0);
+    Soft<A> r = soft_one(Soft<A>{neg_inf<A>(), 0}, rest, c);
+#pragma unroll
+    for (int j = 0; j < HELD; j += U) soft_take<T, E, U>(r, held + j, c);
+    for (int q = HELD * BT + tid; q < run.packs; q += U * BT) {
+        pack<T, E> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = run.template load<!GRAD>(q + u * BT);
+        soft_take<T, E, U>(r, x, c);
+    }
+    soft_leave(r, waves);
+    __syncthreads();
+    const Soft<A> q = soft_collect<BT>(waves);
+    const TeacherSum<A> te = teacher;
+    if (tid < 64) {
+        const A loss = loss_wave(a, q, te, c, p, zk);
+        if (tid == 0) ((A *)a.loss)[a.map.template off<4>(row)] = loss;
+    }
+    if constexpr (GRAD) {
+        const bool zero = te.mass == 0 || w == 0;
+        const A coef = (A)a.temp * w, f = coef * (te.mass / q.s);
+        auto grad = [&](T x) { return zero ? A(0) : f * pow2(fma1((A)x, c, -q.m)); };
+        for (int k = tid; k < a.k; k += BT)
+            if (token[k] >= 0) zk[k] = zero ? A(0) : f * pow2(fma1(zk[k], c, -q.m)) - coef * same_token(a, p, token, k);
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) {
+            keep_whole(held[j]); // (or the sum's conversions to float are kept for this loop, two registers for one)
+            run.store(dz, j * BT + tid, held[j], grad);
+        }
+        for (int i = HELD * BT + tid; i < run.packs; i += U * BT) {
+            pack<T, E> x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = run.template load<true>(i + u * BT);
+#pragma unroll
+            for (int u = 0; u < U; ++u) run.store(dz, i + u * BT, x[u], grad);
+        }
+        run.store_rest(dz, tid, rest, grad);
+        __syncthreads();
+        for (int k = tid; k < a.k; k += BT)
+            if (token[k] >= 0) dz[token[k]] = (T)zk[k];
+    }
 }
 
-// a row's (m, s) from its partials, joined in split order; the same in every thread
-template <class A> DPX_D Soft<A> soft_row(const Distill &a, int64_t row, A c)
+// ---- few rows: split over blocks -------------------------------------------------------------------------------------------
+constexpr int DST_BLOCK = 256;
+// the teacher's side of a row in the workspace: mass, sum p ln p, then p, zk and the tokens' weights
+template <class A> DPX_D A *teacher_part(const Distill &a, int64_t row)
+{
+    return (A *)a.part + a.map.rows * a.splits * 2 + row * (3 * (int64_t)a.k + 2);
+}
+
+// first launch: block (row, split) leaves (M, s) of its part; the last split of a row the teacher's side
+template <class T, class TT> __global__ __launch_bounds__(DST_BLOCK) void distill_split_kernel(Distill a)
+{
+    using A = acc_of<T>;
+    constexpr int E = 16 / (int)sizeof(T), U = 4;
+    extern __shared__ __attribute__((aligned(16))) char raw[];
+    __shared__ Soft<A> waves[DST_BLOCK / 64];
+    A *p = (A *)raw, *zk = p + a.k;
+    int32_t *token = (int32_t *)(zk + a.k);
+    const int64_t row = blockIdx.x / (uint32_t)(a.splits + 1);
+    const int split = (int)(blockIdx.x - (uint32_t)row * (uint32_t)(a.splits + 1)), tid = (int)threadIdx.x;
+    const A c = scale_of<A>(a);
+    if (split == a.splits) { // a block of its own
+        A *to = teacher_part<A>(a, row);
+        if (tid < 64) {
+            const TeacherSum<A> te = teacher_wave<T, TT, A>(a, row, c, p, zk, token);
+            if (tid == 0) {
+                to[0] = te.mass;
+                to[1] = te.plogp;
+            }
+        }
+        __syncthreads();
+        for (int k = tid; k < a.k; k += DST_BLOCK) {
+            to[2 + k] = p[k];
+            to[2 + a.k + k] = zk[k];
+            to[2 + 2 * a.k + k] = same_token(a, p, token, k);
+        }
+        return;
+    }
+    const int begin = (int)(split * a.chunk), end = (int)(begin + a.chunk < a.v ? begin + a.chunk : a.v);
+    const Run<T, E> run((const T *)a.z + a.map.template off<0>(row) + begin, end - begin);
+    Soft<A> r = soft_one(Soft<A>{neg_inf<A>(), 0}, run.load_rest(tid), c);
+    for (int q = tid; q < run.packs; q += U * DST_BLOCK) {
+        pack<T, E> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = run.template load<false>(q + u * DST_BLOCK);
+        soft_take<T, E, U>(r, x, c);
+    }
+    soft_leave(r, waves);
+    __syncthreads();
+    r = soft_collect<DST_BLOCK>(waves);
+    if (tid == 0) ((Soft<A> *)a.part)[row * a.splits + split] = r;
+}
+
+// a row's (M, s) from its parts, the same in every lane: read by the 64 lanes of a wave, joined by DPP
+template <class A> DPX_D Soft<A> soft_row(const Distill &a, int64_t row)
 {
     const Soft<A> *p = (const Soft<A> *)a.part + row * a.splits;
-    Soft<A> r = p[0];
-    for (int k = 1; k < a.splits; ++k) r = soft_join(r, p[k], c);
-    return r;
+    Soft<A> r{neg_inf<A>(), 0};
+    for (int k = threadIdx.x & 63; k < a.splits; k += 64) r = soft_join(r, p[k]);
+    return soft_lanes<64>(r);
 }
 
-template <class T, class TT> __global__ __launch_bounds__(DST_BLOCK) void distill_loss_kernel(Distill a)
+// second launch: the loss, and with GRAD the gradient of block (row, split)'s part
+template <class T, bool GRAD> __global__ __launch_bounds__(GRAD ? DST_BLOCK : 64) void distill_join_kernel(Distill a)
 {
     using A = acc_of<T>;
-    extern __shared__ __attribute__((aligned(16))) char raw[];
-    __shared__ A lds[DST_BLOCK / 64][2];
-    A *p = (A *)raw;
-    int32_t *token = (int32_t *)(p + a.k);
-    const int64_t row = blockIdx.x;
-    const T *z = (const T *)a.z + a.map.template off<0>(row);
-    const A c = (A)(1.4426950408889634074 / a.temp), inv_t = (A)(1.0 / a.temp);
-    const Teacher<A> te = teacher_row<TT, DST_BLOCK, A>(a, row, inv_t, c, p, token, lds);
-    const A loss = row_loss<T, TT, DST_BLOCK>(a, row, z, soft_row<A>(a, row, c), te, inv_t, p, token, lds);
-    if (threadIdx.x == 0) ((A *)a.loss)[a.map.template off<4>(row)] = loss;
-}
-
-// gradient of one chunk of a row.  The gradients at the teacher's tokens are worked out before anything is stored (dz may be
-// z); the dense part is stored first, a barrier, then those few over it.  A row of weight 0, and one without entries, gets
-// zeros whatever its logits are.
-template <class T, class TT> __global__ __launch_bounds__(DST_BLOCK) void distill_grad_kernel(Distill a)
-{
-    using A = acc_of<T>;
-    constexpr int E = 16 / (int)sizeof(T);
-    extern __shared__ __attribute__((aligned(16))) char raw[];
-    __shared__ A lds[DST_BLOCK / 64][2];
-    A *p = (A *)raw, *fix = p + a.k; // the teacher's distribution; the gradient at each of its tokens
-    int32_t *token = (int32_t *)(fix + a.k);
-    const int64_t row = blockIdx.x / (uint32_t)a.splits;
-    const int split = (int)(blockIdx.x - (uint32_t)row * (uint32_t)a.splits);
-    const T *z = (const T *)a.z + a.map.template off<0>(row);
-    T *dz = (T *)a.dz + a.map.template off<5>(row);
-    const int64_t begin = split * a.chunk, end = begin + a.chunk < a.v ? begin + a.chunk : a.v;
-    const A c = (A)(1.4426950408889634074 / a.temp), inv_t = (A)(1.0 / a.temp);
-    const Teacher<A> te = teacher_row<TT, DST_BLOCK, A>(a, row, inv_t, c, p, token, lds);
-    const Soft<A> q = soft_row<A>(a, row, c);
-    const A w = a.wt ? ((const A *)a.wt)[a.map.template off<3>(row)] : A(1);
-    const bool zero = te.mass == 0 || w == 0;
-    const A coef = (A)a.temp * w, qs = te.mass / q.s;
-    for (int k = threadIdx.x; k < a.k; k += DST_BLOCK) {
-        const int32_t i = token[k];
-        if (zero || i < begin || i >= end) continue;
-        A sum = 0; // all entries with this token, in their order
-        for (int j = 0; j < a.k; ++j) sum += token[j] == i ? p[j] : A(0);
-        fix[k] = coef * (pow2(((A)z[i] - q.m) * c) * qs - sum);
+    constexpr int E = 16 / (int)sizeof(T), U = 4;
+    const int splits = GRAD ? a.splits : 1;
+    const int64_t row = blockIdx.x / (uint32_t)splits;
+    const int split = (int)(blockIdx.x - (uint32_t)row * (uint32_t)splits), tid = (int)threadIdx.x;
+    const A c = scale_of<A>(a);
+    const A *te = teacher_part<A>(a, row);
+    const Soft<A> q = soft_row<A>(a, row);
+    if (split == 0 && tid < 64) {
+        const A loss = loss_wave(a, q, TeacherSum<A>{te[0], te[1]}, c, te + 2, te + 2 + a.k);
+        if (tid == 0) ((A *)a.loss)[a.map.template off<4>(row)] = loss;
     }
-    __syncthreads();
-    for (int64_t i = begin + (int64_t)threadIdx.x * E; i < end; i += (int64_t)DST_BLOCK * E) {
-        A x[E];
-        if (i + E <= end) {
-            load_vals<E, false>(z + i, x);
+    if constexpr (GRAD) {
+        const int begin = (int)(split * a.chunk), end = (int)(begin + a.chunk < a.v ? begin + a.chunk : a.v), n = end - begin;
+        const Run<T, E> run((const T *)a.z + a.map.template off<0>(row) + begin, n);
+        T *dz = (T *)a.dz + a.map.template off<5>(row) + begin;
+        const A w = a.wt ? ((const A *)a.wt)[a.map.template off<3>(row)] : A(1);
+        const bool zero = te[0] == 0 || w == 0;
+        const A coef = (A)a.temp * w, f = coef * (te[0] / q.s);
+        auto grad = [&](T x) { return zero ? A(0) : f * pow2(fma1((A)x, c, -q.m)); };
+        run.store_rest(dz, tid, run.load_rest(tid), grad);
+        for (int i = tid; i < run.packs; i += U * DST_BLOCK) {
+            pack<T, E> x[U];
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = zero ? A(0) : coef * (pow2((x[e] - q.m) * c) * qs);
-            store_vals<E, true>(dz + i, x);
+            for (int u = 0; u < U; ++u) x[u] = run.template load<true>(i + u * DST_BLOCK);
+#pragma unroll
+            for (int u = 0; u < U; ++u) run.store(dz, i + u * DST_BLOCK, x[u], grad);
         }
-        else
-            for (int64_t e = i; e < end; ++e) dz[e] = zero ? (T)0 : (T)(coef * (pow2(((A)z[e] - q.m) * c) * qs));
+        __syncthreads();
+        const int64_t to = a.map.template off<2>(row);
+        for (int k = tid; k < a.k; k += DST_BLOCK) {
+            const int64_t i = (a.tok64 ? ((const int64_t *)a.tok)[to + k] : (int64_t)((const int32_t *)a.tok)[to + k]) - begin;
+            if (i >= 0 && i < n)
+                dz[i] = (T)(zero ? A(0) : f * pow2(fma1(te[2 + a.k + k], c, -q.m)) - coef * te[2 + 2 * a.k + k]);
+        }
     }
-    __syncthreads();
-    for (int k = threadIdx.x; k < a.k; k += DST_BLOCK)
-        if (!zero && token[k] >= begin && token[k] < end) dz[token[k]] = (T)fix[k];
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -260,35 +368,53 @@ constexpr int64_t MAX_GRID = 0x7fffffff;
 constexpr int MAX_K = 2048; // the teacher's entries of a row are held in LDS
 
 struct DistillPlan {
-    int splits;
+    int splits; // 0: a block per row
     int64_t chunk;
 };
-// blocks per row: one where the rows alone fill the CUs four times over, else as many as make 1024 blocks, of 4096 elements
-// and more
 DistillPlan distill_plan(int64_t rows, int64_t v)
 {
-    const int64_t want = (int64_t)device_cus() * 4;
-    int64_t splits = rows >= want ? 1 : (want + rows - 1) / rows;
-    splits = std::max<int64_t>(1, std::min(splits, v / 4096));
+    const int64_t cus = device_cus();
+    if (rows >= cus / 2 || v <= 8192) return {0, v};
+    int64_t splits = std::max<int64_t>(1, std::min((cus * 4 + rows - 1) / rows, v / 4096));
     int64_t chunk = (v + splits - 1) / splits;
     chunk = (chunk + 255) / 256 * 256;
     return {(int)((v + chunk - 1) / chunk), chunk};
 }
-int64_t distill_workspace(const dpx_array_view *z)
+int64_t distill_workspace(const dpx_array_view *z, int64_t k)
 {
     if (!view_ok(z) || z->nd < 1 || !row_float(z->dtype) || z->shape[z->nd - 1] == 0) return 0;
     const int64_t v = z->shape[z->nd - 1], rows = view_size(z) / v;
     if (rows == 0) return 0;
-    return rows * distill_plan(rows, v).splits * 2 * itemsize_of(acc_dtype(z->dtype));
+    const DistillPlan pl = distill_plan(rows, v);
+    return pl.splits ? rows * (pl.splits * 2 + 3 * k + 2) * itemsize_of(acc_dtype(z->dtype)) : 0;
 }
 
-template <class T, class TT> int distill_launch(const Distill &a, hipStream_t s)
+template <class T, class TT, bool GRAD> int distill_launch(const Distill &a, hipStream_t s)
 {
     using A = acc_of<T>;
-    const dim3 all((unsigned)(a.map.rows * a.splits)), rows((unsigned)a.map.rows), block(DST_BLOCK);
-    hipLaunchKernelGGL((distill_stats_kernel<T>), all, block, 0, s, a);
-    hipLaunchKernelGGL((distill_loss_kernel<T, TT>), rows, block, (size_t)a.k * (sizeof(A) + 4), s, a);
-    if (a.dz) hipLaunchKernelGGL((distill_grad_kernel<T, TT>), all, block, (size_t)a.k * (2 * sizeof(A) + 4), s, a);
+    constexpr int E = 16 / (int)sizeof(T);
+    const size_t lds = (size_t)a.k * (2 * sizeof(A) + 4);
+    const dim3 rows((unsigned)a.map.rows);
+    if (a.splits == 0) {
+        const int64_t packs = (a.v + E - 1) / E;
+        auto run = [&](auto bt, auto held) {
+            hipLaunchKernelGGL((distill_row_kernel<T, TT, decltype(bt)::value, decltype(held)::value, GRAD>), rows, dim3(bt), lds, s, a);
+        };
+        using std::integral_constant;
+        if constexpr (GRAD) {
+            if (packs <= 1024) run(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+            else if (packs <= 4096) run(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+            else if (packs <= 8192) run(integral_constant<int, 512>{}, integral_constant<int, 16>{});
+            else run(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
+        }
+        else if (packs <= 1024) run(integral_constant<int, 256>{}, integral_constant<int, 0>{});
+        else run(integral_constant<int, 512>{}, integral_constant<int, 0>{});
+    }
+    else {
+        hipLaunchKernelGGL((distill_split_kernel<T, TT>), dim3((unsigned)(a.map.rows * (a.splits + 1))), dim3(DST_BLOCK), lds, s, a);
+        if constexpr (GRAD) hipLaunchKernelGGL((distill_join_kernel<T, true>), dim3((unsigned)(a.map.rows * a.splits)), dim3(DST_BLOCK), 0, s, a);
+        else hipLaunchKernelGGL((distill_join_kernel<T, false>), rows, dim3(64), 0, s, a);
+    }
     const hipError_t rc = hipGetLastError();
     return rc == hipSuccess ? DPX_OK : fail_hip(rc, "distill_topk launch");
 }
@@ -317,21 +443,26 @@ int distill_call(const char *fn, const dpx_array_view *logits, const dpx_array_v
     if (int rc = row_map<6>(fn, args, a.map, p)) return rc;
     if (!(temperature > 0) || !(temperature <= 1e30)) return fail(DPX_ERR_BAD_ARGUMENT, f + "temperature must be a positive number");
     if (a.v == 0) return fail(DPX_ERR_BAD_ARGUMENT, f + "the last axis of logits has no elements");
-    if (a.v > 0x7fffffff) return fail(DPX_ERR_BAD_ARGUMENT, f + "the last axis of logits is too long");
+    if (a.v > 0x3fffffff) return fail(DPX_ERR_BAD_ARGUMENT, f + "the last axis of logits is too long");
     if (k > MAX_K) return fail(DPX_ERR_BAD_ARGUMENT, f + "at most " + std::to_string(MAX_K) + " teacher entries per row");
     if (a.map.rows == 0) return DPX_OK;
     const DistillPlan pl = distill_plan(a.map.rows, a.v);
-    if (a.map.rows * pl.splits > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, f + "too many rows for one launch");
-    const size_t need = (size_t)distill_workspace(logits);
-    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
+    if (a.map.rows * (pl.splits + 1) > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, f + "too many rows for one launch");
+    const size_t need = (size_t)distill_workspace(logits, k);
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return fail(DPX_ERR_BAD_ARGUMENT, f + "a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed");
     a.z = p[0], a.t = p[1], a.tok = p[2], a.wt = p[3], a.loss = p[4], a.dz = p[5];
     a.part = workspace;
     a.chunk = pl.chunk, a.splits = pl.splits, a.k = (int32_t)k, a.tok64 = tokens->dtype == DPX_INT64, a.temp = temperature;
-    if (dt == DPX_HALF && teacher->dtype == DPX_HALF) return distill_launch<half_t, half_t>(a, stream);
-    if (dt == DPX_HALF) return distill_launch<half_t, float>(a, stream);
-    if (dt == DPX_FLOAT) return distill_launch<float, float>(a, stream);
-    return distill_launch<double, double>(a, stream);
+    auto run = [&](auto t, auto u) {
+        using T = typename decltype(t)::type;
+        using TT = typename decltype(u)::type;
+        return grad ? distill_launch<T, TT, true>(a, stream) : distill_launch<T, TT, false>(a, stream);
+    };
+    if (dt == DPX_HALF && teacher->dtype == DPX_HALF) return run(tag<half_t>{}, tag<half_t>{});
+    if (dt == DPX_HALF) return run(tag<half_t>{}, tag<float>{});
+    if (dt == DPX_FLOAT) return run(tag<float>{}, tag<float>{});
+    return run(tag<double>{}, tag<double>{});
 }
 
 } // namespace
@@ -339,7 +470,11 @@ int distill_call(const char *fn, const dpx_array_view *logits, const dpx_array_v
 
 using namespace dpx;
 extern "C" {
-int64_t dpx_distill_topk_workspace(const dpx_array_view *logits) { return distill_workspace(logits); }
+int64_t dpx_distill_topk_workspace(const dpx_array_view *logits, const dpx_array_view *teacher_logits)
+{
+    if (!view_ok(teacher_logits) || teacher_logits->nd < 1) return 0;
+    return distill_workspace(logits, teacher_logits->shape[teacher_logits->nd - 1]);
+}
 int dpx_distill_topk(const dpx_array_view *logits, const dpx_array_view *teacher_logits, const dpx_array_view *teacher_tokens,
                      double temperature, const dpx_array_view *loss, void *workspace, size_t workspace_bytes, void *stream)
 {

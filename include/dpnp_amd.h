@@ -540,7 +540,7 @@ int dpx_layer_norm_grad(const dpx_array_view *grad, const dpx_array_view *x, con
 /* Distillation from a teacher's top logits: loss (acc, the rows' shape) = T^2 KL(p || q) with p = softmax(teacher_logits /
  * T) over a row's entries and q = softmax(logits / T).  teacher_logits: logits' type or acc; teacher_tokens: int32 or
  * int64; both (rows..., K), K <= 2048.  An entry whose token is outside [0, V) is absent; a row with no entry has loss 0. */
-int64_t dpx_distill_topk_workspace(const dpx_array_view *logits);
+int64_t dpx_distill_topk_workspace(const dpx_array_view *logits, const dpx_array_view *teacher_logits);
 int dpx_distill_topk(const dpx_array_view *logits, const dpx_array_view *teacher_logits,
                      const dpx_array_view *teacher_tokens, double temperature, const dpx_array_view *loss, void *workspace,
                      size_t workspace_bytes, void *stream);

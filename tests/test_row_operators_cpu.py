@@ -101,10 +101,13 @@ def test_layer_norm_grad_refusals():
 
 
 def test_distill_refusals():
-    z, t, i, loss, dz = view((3, 100)), view((3, 5)), view((3, 5), L.INT32), view((3,)), view((3, 100))
-    n = lib.dpx_distill_topk_workspace(z)
+    # (three long rows: split over blocks, which need a workspace; a block per row needs none)
+    V = 100000
+    z, t, i, loss, dz = view((3, V)), view((3, 5)), view((3, 5), L.INT32), view((3,)), view((3, V))
+    n = lib.dpx_distill_topk_workspace(z, t)
     ws = ctypes.c_void_p(BASE)
-    assert n > 0 and lib.dpx_distill_topk_workspace(view((0, 100))) == 0
+    assert n > 0 and lib.dpx_distill_topk_workspace(view((0, V)), t) == 0
+    assert lib.dpx_distill_topk_workspace(view((4096, 100)), view((4096, 5))) == 0
 
     def call(z=z, t=t, i=i, w=None, temp=1.0, loss=loss, dz=dz, ws=ws, n=n):
         return lib.dpx_distill_topk_grad(z, t, i, w, temp, loss, dz, ws, n, None)
@@ -114,7 +117,7 @@ def test_distill_refusals():
     refused(lib.dpx_distill_topk(z, t, i, 1.0, loss, ws, 0, None), L.ERR_BAD_ARGUMENT, "workspace")
     for temp in (0.0, -1.0, float("nan"), float("inf")):
         refused(call(temp=temp), L.ERR_BAD_ARGUMENT, "temperature")
-    refused(call(z=view((3, 100), L.INT64)), L.ERR_NOT_IMPLEMENTED, "int64")
+    refused(call(z=view((3, V), L.INT64)), L.ERR_NOT_IMPLEMENTED, "int64")
     refused(call(z=view(())), L.ERR_RANK_MISMATCH, "dimension")
     refused(call(t=view((3, 6))), L.ERR_SHAPE_MISMATCH, "length 5")
     refused(call(t=view((2, 5))), L.ERR_SHAPE_MISMATCH, "leading")
@@ -125,15 +128,15 @@ def test_distill_refusals():
     refused(call(w=view((3, 1))), L.ERR_RANK_MISMATCH, "dimensions")
     refused(call(loss=view((3,), L.HALF)), L.ERR_BAD_DTYPE, "float16")
     refused(call(dz=None), L.ERR_BAD_ARGUMENT, "missing")
-    refused(call(dz=view((3, 100), L.HALF)), L.ERR_BAD_DTYPE, "float16")
-    refused(call(dz=view((3, 100), ptr=z.data + 4)), L.ERR_OVERLAP, "overlap")
-    refused(call(dz=view((3, 100), ptr=t.data)), L.ERR_OVERLAP, "overlap")
+    refused(call(dz=view((3, V), L.HALF)), L.ERR_BAD_DTYPE, "float16")
+    refused(call(dz=view((3, V), ptr=z.data + 4)), L.ERR_OVERLAP, "overlap")
+    refused(call(dz=view((3, V), ptr=t.data)), L.ERR_OVERLAP, "overlap")
     refused(call(loss=view((3,), ptr=z.data)), L.ERR_OVERLAP, "overlap")
     refused(call(t=view((3, 2049)), i=view((3, 2049), L.INT32)), L.ERR_BAD_ARGUMENT, "2048")
     refused(call(z=view((3, 0)), dz=view((3, 0))), L.ERR_BAD_ARGUMENT, "no elements")
     refused(call(z=view((1, 1 << 31)), t=view((1, 5)), i=view((1, 5), L.INT32), loss=view((1,)), dz=view((1, 1 << 31))),
             L.ERR_BAD_ARGUMENT, "too long")
-    assert call(z=view((0, 100)), t=view((0, 5)), i=view((0, 5), L.INT32), loss=view((0,)), dz=view((0, 100)), ws=None, n=0) == L.OK
+    assert call(z=view((0, V)), t=view((0, 5)), i=view((0, 5), L.INT32), loss=view((0,)), dz=view((0, V)), ws=None, n=0) == L.OK
 
 
 def test_process_logits_refusals():
