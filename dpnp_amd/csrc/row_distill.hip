@@ -11,9 +11,16 @@
 // (z_v c - M) ln 2 - ln s, with the same M), so a common offset of the logits costs no accuracy.  Statistics and sums are
 // float32 (float64 for float64 logits).
 //
-// Many rows: a block owns a row.  Its logits are read once, HELD packs per thread stay in registers between the sum and the
-// gradient, what does not fit is read again while it is still in a cache.  Few rows: a row is split over blocks that leave
-// (M, s) in the caller's workspace, and a second launch joins them.
+// A block owns a row.  Its logits are read once, HELD packs per thread stay in registers between the sum and the gradient,
+// what does not fit is read again while it is still in a cache.  Few long rows are split over blocks that leave (M, s) in the
+// caller's workspace, and a second launch joins them.
+//
+// Measured (rocprofv3): gradient of 2048 x 65536 float16 102 us (5.3 TB/s; its exponentials and the rest of its arithmetic
+// take about 50 us of it, which the loads and stores of the other block of the CU hide only in part), of 513 x 100003
+// float32 85 us (one row more than two rounds of the 256 CUs; 512 rows 76), loss of 2048 x 131072 float16 85 us (6.3 TB/s).
+// Tried and not kept: rows that come in while the gradients of the row before go out (persistent blocks, a held pack's
+// registers reloaded after its last use: 160 us, the row's state no longer fits the registers); packs held in LDS as well
+// (158 us for 513 x 100003); a wave of its own for the teacher's side (a block of 9 waves leaves room for one a CU: 111 us).
 #include "row_ops.hpp"
 #include <algorithm>
 
@@ -65,7 +72,7 @@ template <class A> DPX_D void soft_leave(Soft<A> v, Soft<A> *lds)
 template <int BT, class A> DPX_D Soft<A> soft_collect(const Soft<A> *lds)
 {
     constexpr int NW = BT / 64;
-    static_assert(NW == 4 || NW == 8 || NW == 16);
+    static_assert(NW == 2 || NW == 4 || NW == 8 || NW == 16);
     // every row of 16 lanes reads all waves' values (more than once where there are fewer: the duplicates are left out)
     const int lane = threadIdx.x & 15;
     Soft<A> v = lds[lane & (NW - 1)];
@@ -103,11 +110,22 @@ template <class T, int E, int U, class A> DPX_D void soft_take(Soft<A> &r, const
     r.s = (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-// A run of n elements, as packs and fewer than E elements behind them, which the block's first threads take one each.
+// A run of n logits: packs that start on a 128-byte line, and the elements before them (fewer than LINE) and behind them
+// (fewer than E), which the block's first threads take one each.  Rows of an odd length start anywhere, and a wave's 1 KiB
+// of packs then takes one line more and shares it with another wave (512 x 100003 float32: 86 us with packs that are
+// aligned to 16 bytes only, 76 us).  The order of a row's sum thus goes by where the row starts in its line.
 template <class T, int E> struct Run {
-    const T *z;
-    int packs, rest;
-    DPX_D Run(const T *z_, int n) : z(z_), packs(n / E), rest(n % E) {}
+    static constexpr int LINE = 128 / (int)sizeof(T);
+    const T *z; // first pack
+    int head, packs, rest;
+    DPX_D Run(const T *z_, int n)
+    {
+        const int h = (int)((128 - ((uintptr_t)z_ & 127)) & 127) / (int)sizeof(T);
+        head = h < n ? h : n;
+        z = z_ + head;
+        packs = (n - head) / E;
+        rest = (n - head) % E;
+    }
     template <bool NT> DPX_D pack<T, E> load(int p) const // -inf beyond the run
     {
         pack<T, E> x;
@@ -116,8 +134,11 @@ template <class T, int E> struct Run {
         for (int e = 0; e < E; ++e) x.v[e] = (T)(-__builtin_inff());
         return x;
     }
-    DPX_D T load_rest(int i) const { return i < rest ? z[packs * E + i] : (T)(-__builtin_inff()); }
-    // f(z) of every element of pack p
+    // thread i's single element, relative to the first pack; none: -1
+    DPX_D bool single(int i) const { return i < head || (i >= LINE && i < LINE + rest); }
+    DPX_D int single_at(int i) const { return i < LINE ? i - head : packs * E + i - LINE; }
+    DPX_D T load_rest(int i) const { return single(i) ? z[single_at(i)] : (T)(-__builtin_inff()); }
+    // f(z) of every element of pack p; dz: where the first pack goes
     template <class F> DPX_D void store(T *dz, int p, const pack<T, E> &x, F f) const
     {
         acc_of<T> o[E];
@@ -127,7 +148,7 @@ template <class T, int E> struct Run {
     }
     template <class F> DPX_D void store_rest(T *dz, int i, T x, F f) const
     {
-        if (i < rest) dz[packs * E + i] = (T)f(x);
+        if (single(i)) dz[single_at(i)] = (T)f(x);
     }
 };
 template <class T, class A> DPX_D Soft<A> soft_one(Soft<A> r, T x, A c) // one element more
@@ -142,20 +163,31 @@ template <class T, class A> DPX_D Soft<A> soft_one(Soft<A> r, T x, A c) // one e
 template <class A> struct TeacherSum {
     A mass, plogp;
 };
+template <class A> struct TeacherFirst { // entry `lane`, sent for before the row's logits are
+    int64_t token;
+    A t, z;
+};
+template <class T, class TT, class A> DPX_D TeacherFirst<A> teacher_entry(const Distill &a, int64_t row, int k)
+{
+    TeacherFirst<A> f{-1, 0, 0};
+    if (k >= a.k) return f;
+    const int64_t to = a.map.template off<2>(row) + k;
+    f.token = a.tok64 ? ((const int64_t *)a.tok)[to] : (int64_t)((const int32_t *)a.tok)[to];
+    f.t = (A)((const TT *)a.t)[a.map.template off<1>(row) + k];
+    if (f.token >= 0 && f.token < a.v) f.z = (A)((const T *)a.z)[a.map.template off<0>(row) + f.token];
+    return f;
+}
 template <class T, class TT, class A>
-DPX_D TeacherSum<A> teacher_wave(const Distill &a, int64_t row, A c, A *p, A *zk, int32_t *token)
+DPX_D TeacherSum<A> teacher_wave(const Distill &a, int64_t row, A c, TeacherFirst<A> first, A *p, A *zk, int32_t *token)
 {
     const int lane = threadIdx.x & 63;
-    const T *z = (const T *)a.z + a.map.template off<0>(row);
-    const TT *t = (const TT *)a.t + a.map.template off<1>(row);
-    const int64_t to = a.map.template off<2>(row);
     Soft<A> s{neg_inf<A>(), 0};
     for (int k = lane; k < a.k; k += 64) {
-        const int64_t i = a.tok64 ? ((const int64_t *)a.tok)[to + k] : (int64_t)((const int32_t *)a.tok)[to + k];
-        const bool there = i >= 0 && i < a.v;
-        const A x = there ? (A)t[k] : neg_inf<A>();
-        token[k] = there ? (int32_t)i : -1;
-        zk[k] = there ? (A)z[i] : A(0);
+        const TeacherFirst<A> f = k < 64 ? first : teacher_entry<T, TT, A>(a, row, k);
+        const bool there = f.token >= 0 && f.token < a.v;
+        const A x = there ? f.t : neg_inf<A>();
+        token[k] = there ? (int32_t)f.token : -1;
+        zk[k] = f.z;
         p[k] = x;
         const A m = MaxOp{}(s.m, x * c), anc = anchor(m);
         s.s = s.s * pow2(s.m - anc) + pow2(fma1(x, c, -anc));
@@ -191,9 +223,11 @@ template <class A> DPX_D A same_token(const Distill &a, const A *p, const int32_
     return sum;
 }
 
-// ---- many rows: a block owns a row ----------------------------------------------------------------------------------------
-// The gradient is stored densely first, a barrier, then the values at the teacher's tokens over it (their logits were read at
-// the start: dz may be z).  A row of weight 0, and one without entries, gets zeros whatever its logits are.
+// ---- a block owns a row -----------------------------------------------------------------------------------------------
+// HELD packs per thread stay in registers between the sum and the gradient, the others are read again.  The first wave does
+// the teacher's side, whose first entries are sent for before the row.  The gradient is stored densely first, a barrier, then
+// the values at the teacher's tokens over it (their logits were read at the start: dz may be z).  A row of weight 0, and
+// one without entries, gets zeros whatever its logits are.
 template <class T, class TT, int BT, int HELD, bool GRAD>
 __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_kernel(Distill a)
 {
@@ -207,15 +241,18 @@ __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_k
     int32_t *token = (int32_t *)(zk + a.k);
     const int64_t row = blockIdx.x;
     const int tid = (int)threadIdx.x;
-    const Run<T, E> run((const T *)a.z + a.map.template off<0>(row), (int)a.v);
-    T *dz = GRAD ? (T *)a.dz + a.map.template off<5>(row) : nullptr;
     const A c = scale_of<A>(a);
+    const T *z = (const T *)a.z + a.map.template off<0>(row);
+    T *dz = GRAD ? (T *)a.dz + a.map.template off<5>(row) : nullptr;
+    TeacherFirst<A> first{};
+    if (tid < 64) first = teacher_entry<T, TT, A>(a, row, tid);
+    const Run<T, E> run(z, (int)a.v);
     pack<T, E> held[HELD ? HELD : 1];
 #pragma unroll
     for (int j = 0; j < HELD; ++j) held[j] = run.template load<true>(j * BT + tid);
     const T rest = run.load_rest(tid);
     if (tid < 64) {
-        const TeacherSum<A> te = teacher_wave<T, TT, A>(a, row, c, p, zk, token);
+        const TeacherSum<A> te = teacher_wave<T, TT, A>(a, row, c, first, p, zk, token);
         if (tid == 0) teacher = te;
     }
     const A w = GRAD ? (a.wt ? ((const A *)a.wt)[a.map.template off<3>(row)] : A(1)) : A(0);
@@ -242,26 +279,27 @@ __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_k
         auto grad = [&](T x) { return zero ? A(0) : f * pow2(fma1((A)x, c, -q.m)); };
         for (int k = tid; k < a.k; k += BT)
             if (token[k] >= 0) zk[k] = zero ? A(0) : f * pow2(fma1(zk[k], c, -q.m)) - coef * same_token(a, p, token, k);
+        T *to = dz + run.head;
 #pragma unroll
         for (int j = 0; j < HELD; ++j) {
             keep_whole(held[j]); // (or the sum's conversions to float are kept for this loop, two registers for one)
-            run.store(dz, j * BT + tid, held[j], grad);
+            run.store(to, j * BT + tid, held[j], grad);
         }
         for (int i = HELD * BT + tid; i < run.packs; i += U * BT) {
             pack<T, E> x[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) x[u] = run.template load<true>(i + u * BT);
 #pragma unroll
-            for (int u = 0; u < U; ++u) run.store(dz, i + u * BT, x[u], grad);
+            for (int u = 0; u < U; ++u) run.store(to, i + u * BT, x[u], grad);
         }
-        run.store_rest(dz, tid, rest, grad);
+        run.store_rest(to, tid, rest, grad);
         __syncthreads();
         for (int k = tid; k < a.k; k += BT)
             if (token[k] >= 0) dz[token[k]] = (T)zk[k];
     }
 }
 
-// ---- few rows: split over blocks -------------------------------------------------------------------------------------------
+// ---- few long rows: split over blocks -------------------------------------------------------------------------------------------
 constexpr int DST_BLOCK = 256;
 // the teacher's side of a row in the workspace: mass, sum p ln p, then p, zk and the tokens' weights
 template <class A> DPX_D A *teacher_part(const Distill &a, int64_t row)
@@ -284,7 +322,7 @@ template <class T, class TT> __global__ __launch_bounds__(DST_BLOCK) void distil
     if (split == a.splits) { // a block of its own
         A *to = teacher_part<A>(a, row);
         if (tid < 64) {
-            const TeacherSum<A> te = teacher_wave<T, TT, A>(a, row, c, p, zk, token);
+            const TeacherSum<A> te = teacher_wave<T, TT, A>(a, row, c, teacher_entry<T, TT, A>(a, row, tid), p, zk, token);
             if (tid == 0) {
                 to[0] = te.mass;
                 to[1] = te.plogp;
@@ -299,7 +337,8 @@ template <class T, class TT> __global__ __launch_bounds__(DST_BLOCK) void distil
         return;
     }
     const int begin = (int)(split * a.chunk), end = (int)(begin + a.chunk < a.v ? begin + a.chunk : a.v);
-    const Run<T, E> run((const T *)a.z + a.map.template off<0>(row) + begin, end - begin);
+    const T *z = (const T *)a.z + a.map.template off<0>(row) + begin;
+    const Run<T, E> run(z, end - begin);
     Soft<A> r = soft_one(Soft<A>{neg_inf<A>(), 0}, run.load_rest(tid), c);
     for (int q = tid; q < run.packs; q += U * DST_BLOCK) {
         pack<T, E> x[U];
@@ -339,19 +378,20 @@ template <class T, bool GRAD> __global__ __launch_bounds__(GRAD ? DST_BLOCK : 64
     }
     if constexpr (GRAD) {
         const int begin = (int)(split * a.chunk), end = (int)(begin + a.chunk < a.v ? begin + a.chunk : a.v), n = end - begin;
-        const Run<T, E> run((const T *)a.z + a.map.template off<0>(row) + begin, n);
         T *dz = (T *)a.dz + a.map.template off<5>(row) + begin;
+        const Run<T, E> run((const T *)a.z + a.map.template off<0>(row) + begin, n);
+        T *const first = dz + run.head;
         const A w = a.wt ? ((const A *)a.wt)[a.map.template off<3>(row)] : A(1);
         const bool zero = te[0] == 0 || w == 0;
         const A coef = (A)a.temp * w, f = coef * (te[0] / q.s);
         auto grad = [&](T x) { return zero ? A(0) : f * pow2(fma1((A)x, c, -q.m)); };
-        run.store_rest(dz, tid, run.load_rest(tid), grad);
+        run.store_rest(first, tid, run.load_rest(tid), grad);
         for (int i = tid; i < run.packs; i += U * DST_BLOCK) {
             pack<T, E> x[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) x[u] = run.template load<true>(i + u * DST_BLOCK);
 #pragma unroll
-            for (int u = 0; u < U; ++u) run.store(dz, i + u * DST_BLOCK, x[u], grad);
+            for (int u = 0; u < U; ++u) run.store(first, i + u * DST_BLOCK, x[u], grad);
         }
         __syncthreads();
         const int64_t to = a.map.template off<2>(row);
@@ -371,10 +411,16 @@ struct DistillPlan {
     int splits; // 0: a block per row
     int64_t chunk;
 };
-DistillPlan distill_plan(int64_t rows, int64_t v)
+// A block per row is one launch and reads a row once, but a few long rows leave most of the card idle; split rows cost two
+// launches, about 14 us a call.  A call with a block per row / split rows, us (gradient; float16 and float32 within 2 us):
+//   float32  65536 logits   1 row 10.9 / 15.1   64 rows 12.3 / 15.6
+//           131072          1 row 18.1 / 15.2   64 rows 20.8 / 21.5   128 rows 27.9 / 37.6   (loss alone, 64 rows: 18.0 / 13.7)
+//   float64  16384          1 row 15.1 / 15.2   64 rows 19.1 / 15.8   128 rows 19.8 / 18.6
+//           131072          1 row 75.8 / 15.5   64 rows 81.8 / 42.6   128 rows 91.6 / 75.3   200 rows 105 / 116
+DistillPlan distill_plan(int64_t rows, int64_t v, bool is_double)
 {
     const int64_t cus = device_cus();
-    if (rows >= cus / 2 || v <= 8192) return {0, v};
+    if (v <= (is_double ? 24576 : 98304) || rows >= (is_double ? cus * 3 / 4 : cus * 3 / 8)) return {0, v};
     int64_t splits = std::max<int64_t>(1, std::min((cus * 4 + rows - 1) / rows, v / 4096));
     int64_t chunk = (v + splits - 1) / splits;
     chunk = (chunk + 255) / 256 * 256;
@@ -385,7 +431,7 @@ int64_t distill_workspace(const dpx_array_view *z, int64_t k)
     if (!view_ok(z) || z->nd < 1 || !row_float(z->dtype) || z->shape[z->nd - 1] == 0) return 0;
     const int64_t v = z->shape[z->nd - 1], rows = view_size(z) / v;
     if (rows == 0) return 0;
-    const DistillPlan pl = distill_plan(rows, v);
+    const DistillPlan pl = distill_plan(rows, v, z->dtype == DPX_DOUBLE);
     return pl.splits ? rows * (pl.splits * 2 + 3 * k + 2) * itemsize_of(acc_dtype(z->dtype)) : 0;
 }
 
@@ -397,12 +443,14 @@ template <class T, class TT, bool GRAD> int distill_launch(const Distill &a, hip
     const dim3 rows((unsigned)a.map.rows);
     if (a.splits == 0) {
         const int64_t packs = (a.v + E - 1) / E;
+        using std::integral_constant;
         auto run = [&](auto bt, auto held) {
             hipLaunchKernelGGL((distill_row_kernel<T, TT, decltype(bt)::value, decltype(held)::value, GRAD>), rows, dim3(bt), lds, s, a);
         };
-        using std::integral_constant;
         if constexpr (GRAD) {
-            if (packs <= 1024) run(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+            if (packs <= 512) run(integral_constant<int, 128>{}, integral_constant<int, 4>{});
+            else if (packs <= 1024) run(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+            else if (packs <= 2048) run(integral_constant<int, 256>{}, integral_constant<int, 8>{});
             else if (packs <= 4096) run(integral_constant<int, 512>{}, integral_constant<int, 8>{});
             else if (packs <= 8192) run(integral_constant<int, 512>{}, integral_constant<int, 16>{});
             else run(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
@@ -446,7 +494,7 @@ int distill_call(const char *fn, const dpx_array_view *logits, const dpx_array_v
     if (a.v > 0x3fffffff) return fail(DPX_ERR_BAD_ARGUMENT, f + "the last axis of logits is too long");
     if (k > MAX_K) return fail(DPX_ERR_BAD_ARGUMENT, f + "at most " + std::to_string(MAX_K) + " teacher entries per row");
     if (a.map.rows == 0) return DPX_OK;
-    const DistillPlan pl = distill_plan(a.map.rows, a.v);
+    const DistillPlan pl = distill_plan(a.map.rows, a.v, dt == DPX_DOUBLE);
     if (a.map.rows * (pl.splits + 1) > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, f + "too many rows for one launch");
     const size_t need = (size_t)distill_workspace(logits, k);
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))

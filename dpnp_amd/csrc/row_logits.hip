@@ -126,9 +126,9 @@ template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void l
     const T *z = (const T *)a.z + a.map.template off<L_Z>(row);
     T *out = (T *)a.out + a.map.template off<L_OUT>(row);
     const uint8_t *mask = a.mask ? (const uint8_t *)((const uint32_t *)a.mask + a.map.template off<L_MASK>(row)) : nullptr;
-    // the packs are laid so that they are aligned in `out` (rows of an odd length start anywhere): the first one starts `shift`
-    // elements before the row
-    const int shift = (int)((uintptr_t)out / sizeof(T)) & (E - 1);
+    // the packs are laid so that a wave's run of them starts on a 128-byte line of `out` (rows of an odd length start
+    // anywhere): the first one starts `shift` elements before the row
+    const int shift = (int)((uintptr_t)out / sizeof(T)) & (128 / (int)sizeof(T) - 1);
     // a pack's mask bits: two bytes at once, the last ones of the row at most (positions below 0 or past v are not asked for)
     const int mask_last = (v + 31) / 32 * 4 - 2;
     auto mask_byte = [&](int i) { return i >> 3 < mask_last ? i >> 3 : mask_last; };
@@ -265,7 +265,7 @@ constexpr int64_t MAX_GRID = 0x7fffffff;
 
 template <class T, int CHUNK, int BT> int logits_launch_as(Logits &a, int64_t slots, hipStream_t s)
 {
-    a.chunks = (int32_t)((a.v + 16 / sizeof(T) - 1 + CHUNK - 1) / CHUNK); // packs may start before the row
+    a.chunks = (int32_t)((a.v + 128 / sizeof(T) - 1 + CHUNK - 1) / CHUNK); // packs may start before the row
     a.groups = (int32_t)std::max<int64_t>(1, std::min<int64_t>(a.chunks, slots / a.map.rows));
     if (a.map.rows * a.groups > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, "process_logits: too many rows for one launch");
     hipLaunchKernelGGL((logits_kernel<T, CHUNK, BT>), dim3((unsigned)(a.map.rows * a.groups)), dim3(BT), 0, s, a);

@@ -102,7 +102,7 @@ def test_layer_norm_grad_refusals():
 
 def test_distill_refusals():
     # (three long rows: split over blocks, which need a workspace; a block per row needs none)
-    V = 100000
+    V = 200000
     z, t, i, loss, dz = view((3, V)), view((3, 5)), view((3, 5), L.INT32), view((3,)), view((3, V))
     n = lib.dpx_distill_topk_workspace(z, t)
     ws = ctypes.c_void_p(BASE)
