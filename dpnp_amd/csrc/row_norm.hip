@@ -155,35 +155,38 @@ template <class T, class W, int E, int PPL, int G, int BT> __global__ __launch_b
     }
 }
 
-// Rows too long for a block's registers: a block of 1024 threads reads its row three times (the second and third time
-// from the memory-side cache), elements BT apart.
+// Rows too long for a block's registers: blocks of 1024 threads walk down the rows and read each three times (the second
+// and third time from the memory-side cache), elements BT apart.
 template <class T, class W, int BT> __global__ __launch_bounds__(BT) void norm_fwd_long_kernel(NormFwd a)
 {
     using A = acc_of<T>;
-    __shared__ SumPart<1, A> lds[2][BT / 16];
-    const int64_t row = blockIdx.x, n = a.n;
-    const T *x = (const T *)a.x + a.map.template off<0>(row);
-    A s[1] = {0};
-    for (int64_t i = threadIdx.x; i < n; i += BT) s[0] += (A)x[i];
-    row_sums<BT, BT>(s, lds, 0);
-    const A mean = s[0] / (A)n;
-    s[0] = 0;
-    for (int64_t i = threadIdx.x; i < n; i += BT) {
-        const A d = (A)x[i] - mean;
-        s[0] += d * d;
-    }
-    row_sums<BT, BT>(s, lds, 1);
-    const A rstd = A(1) / row_sqrt(s[0] / (A)n + (A)a.eps);
-    T *y = (T *)a.y + a.map.template off<1>(row);
-    for (int64_t i = threadIdx.x; i < n; i += BT) {
-        A o = ((A)x[i] - mean) * rstd;
-        if (a.w) o *= (A)((const W *)a.w)[i];
-        if (a.b) o += (A)((const W *)a.b)[i];
-        y[i] = (T)o;
-    }
-    if (threadIdx.x == 0) {
-        if (a.mean) ((A *)a.mean)[a.map.template off<2>(row)] = mean;
-        if (a.rstd) ((A *)a.rstd)[a.map.template off<3>(row)] = rstd;
+    __shared__ SumPart<1, A> lds[4][BT / 16];
+    const int64_t n = a.n;
+    int slot = 0;
+    for (int64_t row = blockIdx.x; row < a.map.rows; row += gridDim.x, slot ^= 2) {
+        const T *x = (const T *)a.x + a.map.template off<0>(row);
+        A s[1] = {0};
+        for (int64_t i = threadIdx.x; i < n; i += BT) s[0] += (A)x[i];
+        row_sums<BT, BT>(s, lds, slot);
+        const A mean = s[0] / (A)n;
+        s[0] = 0;
+        for (int64_t i = threadIdx.x; i < n; i += BT) {
+            const A d = (A)x[i] - mean;
+            s[0] += d * d;
+        }
+        row_sums<BT, BT>(s, lds, slot + 1);
+        const A rstd = A(1) / row_sqrt(s[0] / (A)n + (A)a.eps);
+        T *y = (T *)a.y + a.map.template off<1>(row);
+        for (int64_t i = threadIdx.x; i < n; i += BT) {
+            A o = ((A)x[i] - mean) * rstd;
+            if (a.w) o *= (A)((const W *)a.w)[i];
+            if (a.b) o += (A)((const W *)a.b)[i];
+            y[i] = (T)o;
+        }
+        if (threadIdx.x == 0) {
+            if (a.mean) ((A *)a.mean)[a.map.template off<2>(row)] = mean;
+            if (a.rstd) ((A *)a.rstd)[a.map.template off<3>(row)] = rstd;
+        }
     }
 }
 

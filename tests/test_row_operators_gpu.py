@@ -91,6 +91,19 @@ def test_layer_norm_rows(shape, dt, wdt):
     check_norm_grad(rng, x, w, mean, rstd)
 
 
+@pytest.mark.parametrize("dt,n", [("f2", 65537), ("f4", 32769), ("f8", 16385)])
+def test_layer_norm_many_long_rows(dt, n):
+    # more rows that do not fit a block's registers than blocks run at once
+    rng = np.random.default_rng(n)
+    few, w, b = norm_data(rng, (13, n), dt, dt)
+    xd, want = dpt.broadcast_to(dev(few), (101, 13, n)), [host(a) for a in check_norm(few, w, b)]
+    out = dpt.full(xd.shape, 7, dtype=dt)
+    y, mean, rstd = dpt.layer_norm(xd, dev(w), dev(b), stats=True, out=out)
+    for got, one in zip((y, mean, rstd), want):
+        got = host(got)
+        assert got.shape == (101,) + one.shape and (got == one).all()
+
+
 @pytest.mark.parametrize("dt", ["f2", "f4", "f8"])
 def test_layer_norm_without_parameters(dt):
     rng = np.random.default_rng(3)
