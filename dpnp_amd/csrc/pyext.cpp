@@ -36,6 +36,7 @@ void *g_stream = nullptr;        // that stream, once known
 PyObject *g_events = nullptr;    // the (event, event) pair of the default queue
 PyObject *g_events_fn = nullptr; // callable(queue) -> (event, event)
 PyObject *g_alloc = nullptr;     // callable(shape tuple, dtype id) -> freshly allocated C-contiguous usm_ndarray
+PyObject *g_alloc_bytes = nullptr; // callable(bytes) -> object with data_ptr()
 PyObject *g_wrap = nullptr;      // callable(usm_ndarray) -> dpnp_array
 
 // result dtype of `op(dt)` / `op(dt, dt)` when the kernel takes the input dtype as it is and the Python
@@ -402,19 +403,33 @@ dpx_array_view *view_or_null(py::handle h, const char *what) { return h.is_none(
 
 // device memory for one call, from the package's allocator: given back in stream order when the object goes
 struct Workspace {
-    py::object array;
+    py::object block;
     void *data = nullptr;
     size_t bytes = 0;
     explicit Workspace(int64_t n)
     {
         if (n <= 0) return;
-        int64_t shape[1] = {n};
-        dpx_array_view *v;
-        array = fresh_result(Py_None, shape, 1, DPX_UINT8, &v);
-        data = v->data;
+        block = py::reinterpret_steal<py::object>(PyObject_CallFunctionObjArgs(g_alloc_bytes, py::int_(n).ptr(), nullptr));
+        if (!block) throw py::error_already_set();
+        data = (void *)py::cast<uintptr_t>(block.attr("data_ptr")());
         bytes = (size_t)n;
     }
 };
+// Whether a kernel may write `out` although it reads `reads` (arrays or None): none overlaps it, but for those of `replaces`
+// that are the same array, element for element.
+bool may_write(py::handle out, py::tuple reads, py::tuple replaces)
+{
+    dpx_array_view *vo = view_arg(out, "out");
+    for (py::handle r : reads) {
+        if (r.is_none()) continue;
+        dpx_array_view *vr = view_arg(r, "operand");
+        if (!dpx_array_overlap(vr, vo)) continue;
+        bool same = false;
+        for (py::handle q : replaces) same = same || (q.ptr() == r.ptr() && dpx_same_logical(vr, vo));
+        if (!same) return false;
+    }
+    return true;
+}
 
 void layer_norm(py::handle x, py::handle weight, py::handle bias, double eps, py::handle y, py::handle mean, py::handle rstd)
 {
@@ -621,6 +636,8 @@ PYBIND11_MODULE(_dpx_ext, m)
         },
         py::arg("src"), py::arg("scalar"), py::arg("dst"), py::arg("sycl_queue") = py::none(),
         py::arg("depends") = py::tuple());
+    m.def("set_alloc_bytes", [](py::object alloc) { g_alloc_bytes = alloc.release().ptr(); });
+    m.def("may_write", &may_write);
     m.def("layer_norm", &layer_norm);
     m.def("layer_norm_grad", &layer_norm_grad);
     m.def("distill_topk", &distill_topk);

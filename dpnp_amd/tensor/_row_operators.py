@@ -11,11 +11,13 @@ import numbers
 from .. import _lib
 from . import _tensor_impl as ti
 from ._copy_utils import copy
+from ._device import alloc
 from ._dtypes import float32, float64
 from ._manipulation_functions import broadcast_to
 from ._usmarray import usm_ndarray
 
 _ext = _lib.ext
+_ext.set_alloc_bytes(alloc)
 
 
 def _array(a, name):
@@ -78,15 +80,7 @@ class _Out:
         if out._dtype != dt:
             raise ValueError(f"Output array of type {dt} is needed for {name}, got {out._dtype}")
         self.user = self.kernel = out
-        direct = not shape or shape[-1] < 2 or out._strides[-1] == 1
-        for a in operands:
-            if a is not None and ti._array_overlap(a, out):
-                for r in replaces:
-                    if a is r and ti._same_logical_tensors(a, out):
-                        break
-                else:
-                    direct = False
-        if not direct:
+        if not ((not shape or shape[-1] < 2 or out._strides[-1] == 1) and _ext.may_write(out, operands, replaces)):
             self.kernel = usm_ndarray._new_contiguous(shape, dt)
 
     def done(self):
@@ -223,7 +217,7 @@ def process_logits(logits, /, *, prompt_tokens=None, prompt_lengths=None, output
     pres = _penalty(presence_penalty, lead, "presence_penalty", 0.0)
     bt, bv = _over_rows(bias_tokens, lead, "bias_tokens"), _over_rows(bias_values, lead, "bias_values")
     ok = _over_rows(allowed, lead, "allowed")
-    reads = () if out is None else [a for a in (z, pt, pl, ot, ol, rep, freq, pres, bt, bv, ok) if type(a) is usm_ndarray]
+    reads = () if out is None else tuple(a for a in (z, pt, pl, ot, ol, rep, freq, pres, bt, bv, ok) if type(a) is usm_ndarray)
     res = _Out(out, z._shape, z._dtype, "out", reads, (z,))
     _ext.process_logits(z, pt, pl, ot, ol, rep, freq, pres, bt, bv, ok, res.kernel)
     return res.done()
