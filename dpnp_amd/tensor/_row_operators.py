@@ -97,6 +97,14 @@ def _several(out, n, what):
     return out
 
 
+def _apart(*outs):
+    """No two results share memory (the kernels' own arrays are checked by the library)."""
+    for i, a in enumerate(outs):
+        for b in outs[:i]:
+            if (a.kernel is not a.user or b.kernel is not b.user) and ti._array_overlap(a.user, b.user):
+                raise ValueError("the arrays of two results overlap in memory")
+
+
 def _acc(dt):
     return float64 if dt == float64 else float32
 
@@ -119,6 +127,7 @@ def layer_norm(x, weight=None, bias=None, /, *, eps=1e-5, stats=False, out=None)
     rows, acc = x._shape[:-1], _acc(x._dtype)
     y = _Out(oy, x._shape, x._dtype, "y", reads, (x,))
     mean, rstd = _Out(om, rows, acc, "mean", reads), _Out(os, rows, acc, "rstd", reads)
+    _apart(y, mean, rstd)
     _ext.layer_norm(x, weight, bias, float(eps), y.kernel, mean.kernel, rstd.kernel)
     return y.done(), mean.done(), rstd.done()
 
@@ -144,6 +153,7 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, /, *, out=None):
         return dx.done(), None, None
     dw = _Out(ow, weight._shape, weight._dtype, "dweight", reads)
     db = _Out(ob, weight._shape, weight._dtype, "dbias", reads)
+    _apart(dx, dw, db)
     _ext.layer_norm_grad(grad, x, mean, rstd, weight, dx.kernel, dw.kernel, db.kernel)
     return dx.done(), dw.done(), db.done()
 
@@ -178,6 +188,7 @@ def distill_topk_grad(logits, teacher_logits, teacher_tokens, weights=None, /, *
     reads = (logits, t, i, w)
     loss = _Out(ol, lead, _acc(logits._dtype), "loss", reads)
     dz = _Out(od, logits._shape, logits._dtype, "dlogits", reads, (logits,))
+    _apart(loss, dz)
     _ext.distill_topk(logits, t, i, w, float(temperature), loss.kernel, dz.kernel)
     return loss.done(), dz.done()
 
@@ -217,7 +228,7 @@ def process_logits(logits, /, *, prompt_tokens=None, prompt_lengths=None, output
     pres = _penalty(presence_penalty, lead, "presence_penalty", 0.0)
     bt, bv = _over_rows(bias_tokens, lead, "bias_tokens"), _over_rows(bias_values, lead, "bias_values")
     ok = _over_rows(allowed, lead, "allowed")
-    reads = () if out is None else tuple(a for a in (z, pt, pl, ot, ol, rep, freq, pres, bt, bv, ok) if type(a) is usm_ndarray)
+    reads = () if out is None else tuple(a for a in (z, pt, pl, ot, ol, rep, freq, pres, bt, bv, ok) if type(a) is not float)
     res = _Out(out, z._shape, z._dtype, "out", reads, (z,))
     _ext.process_logits(z, pt, pl, ot, ol, rep, freq, pres, bt, bv, ok, res.kernel)
     return res.done()

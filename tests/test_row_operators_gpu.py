@@ -567,3 +567,44 @@ def test_row_operators_on_dpnp_arrays():
                             allowed=dpnp.array(d["allowed"]))
     want, tol, _ = ref.process_logits(z, prompt=d["prompt"], rep=1.25, allowed=d["allowed"])
     within(r.asnumpy(), want, tol)
+
+
+def test_rows_beyond_32_bit_offsets():
+    # six rows of an array of 4.6e9 elements: their offsets pass 2^31 and 2^32
+    rng = np.random.default_rng(8)
+    n, every = 65600, 14001
+    far = lambda: dpt.empty((5 * every + 1, n), dtype="f2")[::every]  # noqa: E731
+    x, w, b = norm_data(rng, (6, n), "f2", "f4")
+    xd, out = far(), far()
+    xd[:, :] = dev(x)
+    assert xd.strides[0] * 5 > 2 ** 32
+    for m in (n, 4001):  # the looped kernels and those that hold the row
+        y, mean, rstd = dpt.layer_norm(xd[:, :m], dev(w[:m]), dev(b[:m]), stats=True, out=(out[:, :m], None, None))
+        want = dpt.layer_norm(dev(x[:, :m].copy()), dev(w[:m]), dev(b[:m]), stats=True)
+        for got, one in zip((y, mean, rstd), want):
+            assert np.array_equal(host(got), host(one))
+        got = dpt.layer_norm_grad(y, xd[:, :m], mean, rstd, dev(w[:m]), out=(out[:, :m], None, None))
+        one = dpt.layer_norm_grad(want[0], dev(x[:, :m].copy()), mean, rstd, dev(w[:m]))
+        for g, o in zip(got, one):
+            assert np.array_equal(host(g), host(o))
+    t, tok = rng.standard_normal((6, 9)).astype("f4"), rng.permutation(n)[:54].reshape(6, 9).astype("i4")
+    check_distill(x, t, tok, zd=xd, out=(None, out))
+    tok = dev(tok)
+    got = dpt.process_logits(xd, prompt_tokens=tok, output_tokens=tok, repetition_penalty=1.5, presence_penalty=0.25, out=out)
+    one = dpt.process_logits(dev(x), prompt_tokens=tok, output_tokens=tok, repetition_penalty=1.5, presence_penalty=0.25)
+    assert np.array_equal(host(got), host(one))
+
+
+def test_results_that_share_memory_are_refused():
+    x = dpt.ones((6, 8), dtype="f4")
+    pair = dpt.empty(8, dtype="f4")
+    for out in ((None, pair[:6], pair[:6]), (None, pair[2:], pair[:6]), (x, x[:, 0], None)):
+        with pytest.raises(ValueError, match="overlap"):
+            dpt.layer_norm(x, stats=True, out=out)
+    w = dpt.ones(8, dtype="f4")
+    _, mean, rstd = dpt.layer_norm(x, stats=True)
+    with pytest.raises(ValueError, match="overlap"):
+        dpt.layer_norm_grad(x, x, mean, rstd, w, out=(None, w, w))
+    wide = dpt.empty((6, 16), dtype="f4")
+    with pytest.raises(ValueError, match="overlap"):
+        dpt.distill_topk_grad(x, x[:, :2], dpt.zeros((6, 2), dtype="i4"), out=(wide[:, 2], wide[:, ::2]))
