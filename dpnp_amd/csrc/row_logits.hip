@@ -24,7 +24,7 @@ struct Logits {
     void *out;
     int64_t v;
     int64_t np, no, nb; // entries per row
-    int32_t chunks, groups; // chunks of a row, and blocks that share them
+    int32_t steps, groups; // a row's steps (a pack per thread of a block each), and blocks that share them
     int32_t tok64, btok64;
     double rep0, freq0, pres0; // where no array is given
 };
@@ -105,8 +105,28 @@ template <int BT> struct TokenScan {
     }
 };
 
-// A block takes a run of a row's chunks of CHUNK neighbouring tokens, one after the other, the next chunk's logits on their
-// way.  Per chunk the lists' tokens are counted in LDS words; then every thread looks at the words of its own packs, and
+// A pack's elements whose bit is 0 become -inf: selected by 32-bit words, two float16 at once.
+template <class T, int E> DPX_D void keep_allowed(pack<T, E> &x, uint32_t bits)
+{
+    constexpr int W = E * (int)sizeof(T) / 4;
+    union {
+        pack<T, E> p;
+        uint32_t w[W];
+    } u;
+    u.p = x;
+    auto all = [&](int e) { return (uint32_t)((int32_t)(bits << (31 - e)) >> 31); };
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+        uint32_t keep, inf;
+        if constexpr (sizeof(T) == 2) keep = (all(2 * k) & 0xffffu) | (all(2 * k + 1) & 0xffff0000u), inf = 0xfc00fc00u;
+        else if constexpr (sizeof(T) == 4) keep = all(k), inf = 0xff800000u;
+        else keep = all(k / 2), inf = k & 1 ? 0xfff00000u : 0u;
+        u.w[k] = (u.w[k] & keep) | (inf & ~keep);
+    }
+    x = u.p;
+}
+
+// A block takes a run of a row's steps, CHUNK neighbouring tokens at a time, the next chunk's logits on their way.  Per chunk the lists' tokens are counted in LDS words; then every thread looks at the words of its own packs, and
 // where there are any, puts the pack into its place in LDS and processes the named tokens there one by one (a wave runs as
 // many rounds as the most named pack of its lanes has, mostly one), clears the words, and stores the pack.
 template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void logits_kernel(Logits a)
@@ -121,14 +141,16 @@ template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void l
     __shared__ int bias_count;
     const int64_t row = blockIdx.x / (uint32_t)a.groups;
     const int group = (int)(blockIdx.x - (uint32_t)row * (uint32_t)a.groups), tid = (int)threadIdx.x, v = (int)a.v;
-    int chunk = (int)((int64_t)group * a.chunks / a.groups);
-    const int stop = (int)((int64_t)(group + 1) * a.chunks / a.groups);
     const T *z = (const T *)a.z + a.map.template off<L_Z>(row);
     T *out = (T *)a.out + a.map.template off<L_OUT>(row);
     const uint8_t *mask = a.mask ? (const uint8_t *)((const uint32_t *)a.mask + a.map.template off<L_MASK>(row)) : nullptr;
     // the packs are laid so that a wave's run of them starts on a 128-byte line of `out` (rows of an odd length start
     // anywhere): the first one starts `shift` elements before the row
     const int shift = (int)((uintptr_t)out / sizeof(T)) & (128 / (int)sizeof(T) - 1);
+    // the block's part of the row, in steps of a pack per thread
+    constexpr int STEP = BT * E;
+    int begin = (int)((int64_t)group * a.steps / a.groups) * STEP - shift;
+    const int stop = (int)((int64_t)(group + 1) * a.steps / a.groups) * STEP - shift, end = stop < v ? stop : v;
     // a pack's mask bits: two bytes at once, the last ones of the row at most (positions below 0 or past v are not asked for)
     const int mask_last = (v + 31) / 32 * 4 - 2;
     auto mask_byte = [&](int i) { return i >> 3 < mask_last ? i >> 3 : mask_last; };
@@ -147,22 +169,22 @@ template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void l
         b_token = bias_token(lane);
         b_value = bias_value(lane);
     }
-    auto fetch = [&](int c, pack<T, E>(&x)[PPT], uint32_t(&ok)[PPT]) {
+    auto fetch = [&](int begin, pack<T, E>(&x)[PPT], uint32_t(&ok)[PPT]) {
 #pragma unroll
         for (int j = 0; j < PPT; ++j) {
-            const int i = c * CHUNK - shift + (j * BT + tid) * E;
-            if (i >= 0 && i + E <= v) {
+            const int i = begin + (j * BT + tid) * E;
+            if (i >= 0 && i + E <= end) {
                 x[j] = load_pack<T, E>(z + i);
                 if (mask) ok[j] = load_pack<uint16_t, 1, false>((const uint16_t *)(mask + mask_byte(i))).v[0];
             }
             else
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[j].v[e] = i + e >= 0 && i + e < v ? z[i + e] : (T)0;
+                for (int e = 0; e < E; ++e) x[j].v[e] = i + e >= 0 && i + e < end ? z[i + e] : (T)0;
         }
     };
     pack<T, E> x[PPT], x2[PPT];
     uint32_t ok[PPT], ok2[PPT];
-    fetch(chunk, x, ok);
+    fetch(begin, x, ok);
     const bool lists = a.prompt || a.output || a.btok;
     const A rep = a.rep ? (A)((const float *)a.rep)[a.map.template off<L_REP>(row)] : (A)a.rep0;
     const A freq = a.freq ? (A)((const float *)a.freq)[a.map.template off<L_FREQ>(row)] : (A)a.freq0;
@@ -172,9 +194,9 @@ template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void l
     if (lists)
         for (int i = tid * 4; i < CHUNK; i += BT * 4) *(u32x4 *)(word + i) = u32x4{0, 0, 0, 0};
     T *mine = value + tid * E;
-    for (; chunk < stop; ++chunk) {
-        const int begin = chunk * CHUNK - shift, n = v - begin < CHUNK ? v - begin : CHUNK;
-        if (chunk + 1 < stop) fetch(chunk + 1, x2, ok2);
+    for (; begin < end; begin += CHUNK) {
+        const int n = end - begin < CHUNK ? end - begin : CHUNK;
+        if (begin + CHUNK < end) fetch(begin + CHUNK, x2, ok2);
         if (lists) {
             __syncthreads(); // the words are clear
             prompt.take(begin, n, [&](int t) { atomicOr(&word[t], SEEN_PROMPT); });
@@ -244,11 +266,7 @@ template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void l
             }
             const int g = begin + i;
             if (g >= 0 && i + E <= n) {
-                if (mask) {
-                    const uint32_t bits = ok[j] >> (g - 8 * mask_byte(g));
-#pragma unroll
-                    for (int e = 0; e < E; ++e) x[j].v[e] = (bits >> e) & 1 ? x[j].v[e] : (T)(-__builtin_inff());
-                }
+                if (mask) keep_allowed(x[j], ok[j] >> (g - 8 * mask_byte(g)));
                 store_pack<T, E>(out + g, x[j]);
             }
             else
@@ -265,21 +283,26 @@ constexpr int64_t MAX_GRID = 0x7fffffff;
 
 template <class T, int CHUNK, int BT> int logits_launch_as(Logits &a, int64_t slots, hipStream_t s)
 {
-    a.chunks = (int32_t)((a.v + 128 / sizeof(T) - 1 + CHUNK - 1) / CHUNK); // packs may start before the row
-    a.groups = (int32_t)std::max<int64_t>(1, std::min<int64_t>(a.chunks, slots / a.map.rows));
+    constexpr int64_t STEP = BT * (16 / (int)sizeof(T));
+    const int64_t span = a.v + 128 / (int64_t)sizeof(T) - 1; // packs may start before the row
+    a.steps = (int32_t)((span + STEP - 1) / STEP);
+    a.groups = (int32_t)std::max<int64_t>(1, std::min<int64_t>((span + CHUNK - 1) / CHUNK, slots / a.map.rows));
     if (a.map.rows * a.groups > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, "process_logits: too many rows for one launch");
     hipLaunchKernelGGL((logits_kernel<T, CHUNK, BT>), dim3((unsigned)(a.map.rows * a.groups)), dim3(BT), 0, s, a);
     const hipError_t rc = hipGetLastError();
     return rc == hipSuccess ? DPX_OK : fail_hip(rc, "process_logits launch");
 }
-// Chunks and blocks.  With many rows: 8192 tokens by 512 threads (float64: 2048, whose registers spill beyond), three blocks a
-// CU that share out each row's chunks and keep the next chunk's logits in flight while they count (256 rows of 100003
-// float16, lists of 1800 and 700 tokens, 50 biases, mask: 28.9 us; a block per chunk, which reads the lists anew and has
+// Chunks and blocks.  With many rows: a chunk of two packs per thread of 512 (float32: three; more spill), three blocks a CU
+// that share out each row's steps and keep the next chunk's logits in flight while they count (256 rows of 100003 float16,
+// lists of 1800 and 700 tokens, 50 biases, mask: 27.9 us, 3.8 TB/s; a block per chunk, which reads the lists anew and has
 // nothing in flight meanwhile: 38.7; 4096 tokens by 256 threads: 30.3).  Without lists there is nothing to keep: a block per
-// chunk streams better (mask alone 22.8 against 24.8 us).  With few rows small chunks, so that the row is spread over the CUs.
+// chunk streams better (mask alone 22.8 against 24.8 us).  With few rows small chunks, so that the row is spread over the CUs
+// (1 row of 131072 float32, lists of 700 and 300 tokens: 5.6 us).
+// Letting the threads that hold a token process it in LDS, instead of the thread that holds the logit: 28.4 and 6.4 us
+// (one more barrier), 44 against 50 for 1024 rows of 32000, where one token in 13 is named.
 template <class T> int logits_launch(Logits &a, hipStream_t s)
 {
-    constexpr int E = 16 / (int)sizeof(T), CHUNK = sizeof(T) == 8 ? 2048 : 8192;
+    constexpr int E = 16 / (int)sizeof(T), CHUNK = 512 * E * (sizeof(T) == 4 ? 3 : 2);
     const int64_t cus = device_cus(), many = (int64_t)1 << 40;
     const bool lists = a.prompt || a.output || a.btok;
     if (a.map.rows * ((a.v + CHUNK - 1) / CHUNK) >= cus * 2) return logits_launch_as<T, CHUNK, 512>(a, lists ? cus * 3 : many, s);
