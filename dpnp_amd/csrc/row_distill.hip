@@ -34,6 +34,7 @@ struct Distill {
     void *part; // split rows: [rows][splits] pairs (M, s), then [rows][3 k + 2] values of the teacher's side
     int64_t v, chunk;
     int32_t k, tok64, splits;
+    int32_t table; // gradient: size of the token table
     double temp;
 };
 
@@ -162,33 +163,75 @@ template <class T, class A> DPX_D Soft<A> soft_one(Soft<A> r, T x, A c) // one e
 // mass sum(p) (1, 0 with no entry that counts, or NaN) and sum p ln p.
 template <class A> struct TeacherSum {
     A mass, plogp;
+    bool repeats; // some token belongs to several entries
 };
-template <class A> struct TeacherFirst { // entry `lane`, sent for before the row's logits are
-    int64_t token;
+// The row's tokens in a hash table in LDS (open addressing, at most a quarter full), which tells those of several entries:
+// comparing every entry with all others took a block 8 us for 256 entries and 200 us for 1000 more than this.
+constexpr uint32_t FREE = ~0u, REPEATED = 1u << 31;
+constexpr int table_size(int k)
+{
+    int n = 64;
+    while (n < 4 * k) n *= 2;
+    return n;
+}
+DPX_D uint32_t table_start(uint32_t token) { return (token * 2654435761u) >> 16; } // (2^32 / the golden ratio)
+DPX_D bool table_put(uint32_t *table, int n, uint32_t token) // true: it was there already
+{
+    for (uint32_t at = table_start(token);; ++at) {
+        uint32_t *const slot = table + (at & (uint32_t)(n - 1));
+        const uint32_t old = atomicCAS(slot, FREE, token);
+        if (old == FREE) return false;
+        if ((old & ~REPEATED) == token) {
+            atomicOr(slot, REPEATED);
+            return true;
+        }
+    }
+}
+DPX_D bool table_repeated(const uint32_t *table, int n, uint32_t token) // of a token that is there
+{
+    for (uint32_t at = table_start(token);; ++at) {
+        const uint32_t w = table[at & (uint32_t)(n - 1)];
+        if ((w & ~REPEATED) == token) return (w & REPEATED) != 0;
+    }
+}
+template <class A> struct Entry {
+    int32_t token; // -1: absent
     A t, z;
 };
-template <class T, class TT, class A> DPX_D TeacherFirst<A> teacher_entry(const Distill &a, int64_t row, int k)
+template <class T, class TT, class A> DPX_D Entry<A> teacher_entry(const Distill &a, int64_t row, int k)
 {
-    TeacherFirst<A> f{-1, 0, 0};
+    Entry<A> f{-1, 0, 0};
     if (k >= a.k) return f;
     const int64_t to = a.map.template off<2>(row) + k;
-    f.token = a.tok64 ? ((const int64_t *)a.tok)[to] : (int64_t)((const int32_t *)a.tok)[to];
+    const int64_t token = a.tok64 ? ((const int64_t *)a.tok)[to] : (int64_t)((const int32_t *)a.tok)[to];
     f.t = (A)((const TT *)a.t)[a.map.template off<1>(row) + k];
-    if (f.token >= 0 && f.token < a.v) f.z = (A)((const T *)a.z)[a.map.template off<0>(row) + f.token];
+    if (token >= 0 && token < a.v) {
+        f.token = (int32_t)token;
+        f.z = (A)((const T *)a.z)[a.map.template off<0>(row) + token];
+    }
     return f;
 }
-template <class T, class TT, class A>
-DPX_D TeacherSum<A> teacher_wave(const Distill &a, int64_t row, A c, TeacherFirst<A> first, A *p, A *zk, int32_t *token)
+template <class T, class TT, bool GRAD, class A>
+DPX_D TeacherSum<A> teacher_wave(const Distill &a, int64_t row, A c, Entry<A> first, A *p, A *zk, int32_t *token)
 {
     const int lane = threadIdx.x & 63;
+    uint32_t *const table = (uint32_t *)(token + a.k);
+    if constexpr (GRAD) {
+        for (int i = lane; i < a.table; i += 64) table[i] = FREE;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); // (the wave's LDS accesses are done in order)
+        __builtin_amdgcn_wave_barrier();
+    }
+    bool repeats = false;
     Soft<A> s{neg_inf<A>(), 0};
     for (int k = lane; k < a.k; k += 64) {
-        const TeacherFirst<A> f = k < 64 ? first : teacher_entry<T, TT, A>(a, row, k);
-        const bool there = f.token >= 0 && f.token < a.v;
+        const Entry<A> f = k < 64 ? first : teacher_entry<T, TT, A>(a, row, k);
+        const bool there = f.token >= 0;
         const A x = there ? f.t : neg_inf<A>();
-        token[k] = there ? (int32_t)f.token : -1;
+        token[k] = f.token;
         zk[k] = f.z;
         p[k] = x;
+        if constexpr (GRAD)
+            if (there) repeats |= table_put(table, a.table, (uint32_t)f.token);
         const A m = MaxOp{}(s.m, x * c), anc = anchor(m);
         s.s = s.s * pow2(s.m - anc) + pow2(fma1(x, c, -anc));
         s.m = m;
@@ -202,7 +245,7 @@ DPX_D TeacherSum<A> teacher_wave(const Distill &a, int64_t row, A c, TeacherFirs
         p[k] = pk;
         if (pk != 0) plogp += pk * (e * (A)0.69314718055994530942 - lns);
     }
-    return {none ? A(0) : s.s * inv, lanes_fold<64>(plogp, SumOp{})};
+    return {none ? A(0) : s.s * inv, lanes_fold<64>(plogp, SumOp{}), __builtin_amdgcn_ballot_w64(repeats) != 0};
 }
 // loss of the row from the student's (M, s): by one wave
 template <class A> DPX_D A loss_wave(const Distill &a, Soft<A> q, TeacherSum<A> te, A c, const A *p, const A *zk)
@@ -215,10 +258,12 @@ template <class A> DPX_D A loss_wave(const Distill &a, Soft<A> q, TeacherSum<A> 
     return te.mass == 0 ? A(0) : (A)(a.temp * a.temp) * (te.plogp - sum);
 }
 // all the weight that entry k's token gets, its own and that of other entries with the same token, in their order
-template <class A> DPX_D A same_token(const Distill &a, const A *p, const int32_t *token, int k)
+template <class A> DPX_D A token_weight(const Distill &a, bool repeats, const A *p, const int32_t *token, int k)
 {
     const int32_t i = token[k];
+    if (!repeats || i < 0 || !table_repeated((const uint32_t *)(token + a.k), a.table, (uint32_t)i)) return p[k];
     A sum = 0;
+#pragma unroll 8
     for (int j = 0; j < a.k; ++j) sum += token[j] == i ? p[j] : A(0);
     return sum;
 }
@@ -244,7 +289,7 @@ __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_k
     const A c = scale_of<A>(a);
     const T *z = (const T *)a.z + a.map.template off<0>(row);
     T *dz = GRAD ? (T *)a.dz + a.map.template off<5>(row) : nullptr;
-    TeacherFirst<A> first{};
+    Entry<A> first{};
     if (tid < 64) first = teacher_entry<T, TT, A>(a, row, tid);
     const Run<T, E> run(z, (int)a.v);
     pack<T, E> held[HELD ? HELD : 1];
@@ -252,7 +297,7 @@ __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_k
     for (int j = 0; j < HELD; ++j) held[j] = run.template load<true>(j * BT + tid);
     const T rest = run.load_rest(tid);
     if (tid < 64) {
-        const TeacherSum<A> te = teacher_wave<T, TT, A>(a, row, c, first, p, zk, token);
+        const TeacherSum<A> te = teacher_wave<T, TT, GRAD>(a, row, c, first, p, zk, token);
         if (tid == 0) teacher = te;
     }
     const A w = GRAD ? (a.wt ? ((const A *)a.wt)[a.map.template off<3>(row)] : A(1)) : A(0);
@@ -269,16 +314,14 @@ __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_k
     __syncthreads();
     const Soft<A> q = soft_collect<BT>(waves);
     const TeacherSum<A> te = teacher;
-    if (tid < 64) {
+    if (tid >= BT - 64) {
         const A loss = loss_wave(a, q, te, c, p, zk);
-        if (tid == 0) ((A *)a.loss)[a.map.template off<4>(row)] = loss;
+        if (tid == BT - 64) ((A *)a.loss)[a.map.template off<4>(row)] = loss;
     }
     if constexpr (GRAD) {
         const bool zero = te.mass == 0 || w == 0;
         const A coef = (A)a.temp * w, f = coef * (te.mass / q.s);
         auto grad = [&](T x) { return zero ? A(0) : f * pow2(fma1((A)x, c, -q.m)); };
-        for (int k = tid; k < a.k; k += BT)
-            if (token[k] >= 0) zk[k] = zero ? A(0) : f * pow2(fma1(zk[k], c, -q.m)) - coef * same_token(a, p, token, k);
         T *to = dz + run.head;
 #pragma unroll
         for (int j = 0; j < HELD; ++j) {
@@ -295,7 +338,8 @@ __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_k
         run.store_rest(to, tid, rest, grad);
         __syncthreads();
         for (int k = tid; k < a.k; k += BT)
-            if (token[k] >= 0) dz[token[k]] = (T)zk[k];
+            if (token[k] >= 0)
+                dz[token[k]] = (T)(zero ? A(0) : f * pow2(fma1(zk[k], c, -q.m)) - coef * token_weight(a, te.repeats, p, token, k));
     }
 }
 
@@ -308,12 +352,13 @@ template <class A> DPX_D A *teacher_part(const Distill &a, int64_t row)
 }
 
 // first launch: block (row, split) leaves (M, s) of its part; the last split of a row the teacher's side
-template <class T, class TT> __global__ __launch_bounds__(DST_BLOCK) void distill_split_kernel(Distill a)
+template <class T, class TT, bool GRAD> __global__ __launch_bounds__(DST_BLOCK) void distill_split_kernel(Distill a)
 {
     using A = acc_of<T>;
     constexpr int E = 16 / (int)sizeof(T), U = 4;
     extern __shared__ __attribute__((aligned(16))) char raw[];
     __shared__ Soft<A> waves[DST_BLOCK / 64];
+    __shared__ bool repeats;
     A *p = (A *)raw, *zk = p + a.k;
     int32_t *token = (int32_t *)(zk + a.k);
     const int64_t row = blockIdx.x / (uint32_t)(a.splits + 1);
@@ -322,17 +367,18 @@ template <class T, class TT> __global__ __launch_bounds__(DST_BLOCK) void distil
     if (split == a.splits) { // a block of its own
         A *to = teacher_part<A>(a, row);
         if (tid < 64) {
-            const TeacherSum<A> te = teacher_wave<T, TT, A>(a, row, c, teacher_entry<T, TT, A>(a, row, tid), p, zk, token);
+            const TeacherSum<A> te = teacher_wave<T, TT, GRAD>(a, row, c, teacher_entry<T, TT, A>(a, row, tid), p, zk, token);
             if (tid == 0) {
                 to[0] = te.mass;
                 to[1] = te.plogp;
+                repeats = te.repeats;
             }
         }
         __syncthreads();
         for (int k = tid; k < a.k; k += DST_BLOCK) {
             to[2 + k] = p[k];
             to[2 + a.k + k] = zk[k];
-            to[2 + 2 * a.k + k] = same_token(a, p, token, k);
+            if constexpr (GRAD) to[2 + 2 * a.k + k] = token_weight(a, repeats, p, token, k);
         }
         return;
     }
@@ -371,34 +417,52 @@ template <class T, bool GRAD> __global__ __launch_bounds__(GRAD ? DST_BLOCK : 64
     const int split = (int)(blockIdx.x - (uint32_t)row * (uint32_t)splits), tid = (int)threadIdx.x;
     const A c = scale_of<A>(a);
     const A *te = teacher_part<A>(a, row);
-    const Soft<A> q = soft_row<A>(a, row);
-    if (split == 0 && tid < 64) {
-        const A loss = loss_wave(a, q, TeacherSum<A>{te[0], te[1]}, c, te + 2, te + 2 + a.k);
-        if (tid == 0) ((A *)a.loss)[a.map.template off<4>(row)] = loss;
-    }
-    if constexpr (GRAD) {
+    auto loss = [&](Soft<A> q) {
+        if (split != 0 || tid >= 64) return;
+        const A l = loss_wave(a, q, TeacherSum<A>{te[0], te[1], false}, c, te + 2, te + 2 + a.k);
+        if (tid == 0) ((A *)a.loss)[a.map.template off<4>(row)] = l;
+    };
+    if constexpr (!GRAD) loss(soft_row<A>(a, row));
+    else {
+        // everything that does not wait for the row's sum is sent for before it
         const int begin = (int)(split * a.chunk), end = (int)(begin + a.chunk < a.v ? begin + a.chunk : a.v), n = end - begin;
         T *dz = (T *)a.dz + a.map.template off<5>(row) + begin;
         const Run<T, E> run((const T *)a.z + a.map.template off<0>(row) + begin, n);
         T *const first = dz + run.head;
-        const A w = a.wt ? ((const A *)a.wt)[a.map.template off<3>(row)] : A(1);
-        const bool zero = te[0] == 0 || w == 0;
-        const A coef = (A)a.temp * w, f = coef * (te[0] / q.s);
-        auto grad = [&](T x) { return zero ? A(0) : f * pow2(fma1((A)x, c, -q.m)); };
-        run.store_rest(first, tid, run.load_rest(tid), grad);
-        for (int i = tid; i < run.packs; i += U * DST_BLOCK) {
-            pack<T, E> x[U];
+        pack<T, E> x[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) x[u] = run.template load<true>(i + u * DST_BLOCK);
+        for (int u = 0; u < U; ++u) x[u] = run.template load<true>(tid + u * DST_BLOCK);
+        const T one = run.load_rest(tid);
+        const int64_t to = a.map.template off<2>(row);
+        struct Named {
+            int64_t at;
+            A z, weight;
+        };
+        auto entry = [&](int k) {
+            if (k >= a.k) return Named{-1, 0, 0};
+            const int64_t token = a.tok64 ? ((const int64_t *)a.tok)[to + k] : (int64_t)((const int32_t *)a.tok)[to + k];
+            return Named{token - begin, te[2 + a.k + k], te[2 + 2 * a.k + k]};
+        };
+        const Named mine = entry(tid);
+        const A w = a.wt ? ((const A *)a.wt)[a.map.template off<3>(row)] : A(1), mass = te[0];
+        const Soft<A> q = soft_row<A>(a, row);
+        const bool zero = mass == 0 || w == 0;
+        const A coef = (A)a.temp * w, f = coef * (mass / q.s);
+        auto grad = [&](T x) { return zero ? A(0) : f * pow2(fma1((A)x, c, -q.m)); };
+        run.store_rest(first, tid, one, grad);
+        for (int i = tid;;) {
 #pragma unroll
             for (int u = 0; u < U; ++u) run.store(first, i + u * DST_BLOCK, x[u], grad);
+            i += U * DST_BLOCK;
+            if (i >= run.packs) break;
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = run.template load<true>(i + u * DST_BLOCK);
         }
+        loss(q);
         __syncthreads();
-        const int64_t to = a.map.template off<2>(row);
         for (int k = tid; k < a.k; k += DST_BLOCK) {
-            const int64_t i = (a.tok64 ? ((const int64_t *)a.tok)[to + k] : (int64_t)((const int32_t *)a.tok)[to + k]) - begin;
-            if (i >= 0 && i < n)
-                dz[i] = (T)(zero ? A(0) : f * pow2(fma1(te[2 + a.k + k], c, -q.m)) - coef * te[2 + 2 * a.k + k]);
+            const Named t = k < DST_BLOCK ? mine : entry(k);
+            if (t.at >= 0 && t.at < n) dz[t.at] = (T)(zero ? A(0) : f * pow2(fma1(t.z, c, -q.m)) - coef * t.weight);
         }
     }
 }
@@ -439,7 +503,7 @@ template <class T, class TT, bool GRAD> int distill_launch(const Distill &a, hip
 {
     using A = acc_of<T>;
     constexpr int E = 16 / (int)sizeof(T);
-    const size_t lds = (size_t)a.k * (2 * sizeof(A) + 4);
+    const size_t lds = (size_t)a.k * (2 * sizeof(A) + 4) + (size_t)a.table * 4;
     const dim3 rows((unsigned)a.map.rows);
     if (a.splits == 0) {
         const int64_t packs = (a.v + E - 1) / E;
@@ -459,7 +523,7 @@ template <class T, class TT, bool GRAD> int distill_launch(const Distill &a, hip
         else run(integral_constant<int, 512>{}, integral_constant<int, 0>{});
     }
     else {
-        hipLaunchKernelGGL((distill_split_kernel<T, TT>), dim3((unsigned)(a.map.rows * (a.splits + 1))), dim3(DST_BLOCK), lds, s, a);
+        hipLaunchKernelGGL((distill_split_kernel<T, TT, GRAD>), dim3((unsigned)(a.map.rows * (a.splits + 1))), dim3(DST_BLOCK), lds, s, a);
         if constexpr (GRAD) hipLaunchKernelGGL((distill_join_kernel<T, true>), dim3((unsigned)(a.map.rows * a.splits)), dim3(DST_BLOCK), 0, s, a);
         else hipLaunchKernelGGL((distill_join_kernel<T, false>), rows, dim3(64), 0, s, a);
     }
@@ -502,6 +566,7 @@ int distill_call(const char *fn, const dpx_array_view *logits, const dpx_array_v
     a.z = p[0], a.t = p[1], a.tok = p[2], a.wt = p[3], a.loss = p[4], a.dz = p[5];
     a.part = workspace;
     a.chunk = pl.chunk, a.splits = pl.splits, a.k = (int32_t)k, a.tok64 = tokens->dtype == DPX_INT64, a.temp = temperature;
+    a.table = grad ? table_size((int)k) : 0;
     auto run = [&](auto t, auto u) {
         using T = typename decltype(t)::type;
         using TT = typename decltype(u)::type;

@@ -300,6 +300,20 @@ def test_distill_absent_repeated_and_empty(v, dt):
 
 
 @pytest.mark.parametrize("dt", ["f2", "f4", "f8"])
+@pytest.mark.parametrize("v", [600, 40000, 140001])
+@pytest.mark.parametrize("k", [63, 65, 257, 2048])
+def test_distill_many_entries_some_repeated(v, k, dt):
+    rng = np.random.default_rng(k)
+    z, t, tok = distill_data(rng, 6, v, k, dt)
+    tok[0] = rng.integers(0, v, k)          # as they fall
+    tok[1] = rng.integers(0, 5, k) * 64     # few tokens, neighbours in a table of a power of two
+    tok[2, k // 2:] = tok[2, :k - k // 2]   # each twice, far apart
+    tok[3, 1:] = -1                         # one entry and none else
+    tok[4] = np.arange(k) % v               # one after the other
+    check_distill(z, t, tok)
+
+
+@pytest.mark.parametrize("dt", ["f2", "f4", "f8"])
 @pytest.mark.parametrize("v", [40, 70000])
 def test_distill_special_values(v, dt):
     """What NaN and infinities in the logits, the teacher and the weights come to, row by row."""
