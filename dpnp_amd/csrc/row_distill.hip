@@ -476,15 +476,21 @@ struct DistillPlan {
     int64_t chunk;
 };
 // A block per row is one launch and reads a row once, but a few long rows leave most of the card idle; split rows cost two
-// launches, about 14 us a call.  A call with a block per row / split rows, us (gradient; float16 and float32 within 2 us):
-//   float32  65536 logits   1 row 10.9 / 15.1   64 rows 12.3 / 15.6
-//           131072          1 row 18.1 / 15.2   64 rows 20.8 / 21.5   128 rows 27.9 / 37.6   (loss alone, 64 rows: 18.0 / 13.7)
-//   float64  16384          1 row 15.1 / 15.2   64 rows 19.1 / 15.8   128 rows 19.8 / 18.6
-//           131072          1 row 75.8 / 15.5   64 rows 81.8 / 42.6   128 rows 91.6 / 75.3   200 rows 105 / 116
-DistillPlan distill_plan(int64_t rows, int64_t v, bool is_double)
+// launches, about 11 us a call.  A call with a block per row / split rows, us (float16 and float32 within 4 us):
+//                            1 row         64 rows       96 rows       128 rows      192 rows
+//   float32  65536 gradient   9.3 / 13.2   13.1 / 14.8   loss 1 row 7.6 / 11.0, 64 rows 10.4 / 11.3
+//           131072 gradient  19.0 / 12.2   21.5 / 20.8   23.3 / 29.0   28.9 / 37.2
+//                  loss      16.0 / 10.7   17.3 / 11.2   18.0 / 15.2   18.4 / 18.5
+//   float64  12288 gradient  13.9 / 12.2   17.7 / 14.0   loss 1 row  7.5 / 10.2, 64 rows 8.9 / 10.4
+//            16384 gradient  15.6 / 11.6   17.8 / 15.3                 18.8 / 18.3
+//                  loss       9.2 / 10.2   10.0 / 10.6                  9.9 / 11.2
+//           131072 gradient  76.1 / 11.7   81.5 / 42.1                 91.6 / 75.3   106 / 115
+//                  loss      44.1 / 10.3   46.3 / 21.9                               48.7 / 53.2
+DistillPlan distill_plan(int64_t rows, int64_t v, bool is_double, bool grad)
 {
     const int64_t cus = device_cus();
-    if (v <= (is_double ? 24576 : 98304) || rows >= (is_double ? cus * 3 / 4 : cus * 3 / 8)) return {0, v};
+    if (v <= (!is_double ? 90112 : grad ? 10240 : 18432)) return {0, v};
+    if (rows > (is_double ? cus * 5 / 8 : grad ? cus / 4 : cus / 2)) return {0, v};
     int64_t splits = std::max<int64_t>(1, std::min((cus * 4 + rows - 1) / rows, v / 4096));
     int64_t chunk = (v + splits - 1) / splits;
     chunk = (chunk + 255) / 256 * 256;
@@ -495,8 +501,9 @@ int64_t distill_workspace(const dpx_array_view *z, int64_t k)
     if (!view_ok(z) || z->nd < 1 || !row_float(z->dtype) || z->shape[z->nd - 1] == 0) return 0;
     const int64_t v = z->shape[z->nd - 1], rows = view_size(z) / v;
     if (rows == 0) return 0;
-    const DistillPlan pl = distill_plan(rows, v, z->dtype == DPX_DOUBLE);
-    return pl.splits ? rows * (pl.splits * 2 + 3 * k + 2) * itemsize_of(acc_dtype(z->dtype)) : 0;
+    const bool is_double = z->dtype == DPX_DOUBLE; // (one size for the loss alone and with its gradient)
+    const int64_t splits = std::max(distill_plan(rows, v, is_double, false).splits, distill_plan(rows, v, is_double, true).splits);
+    return splits ? rows * (splits * 2 + 3 * k + 2) * itemsize_of(acc_dtype(z->dtype)) : 0;
 }
 
 template <class T, class TT, bool GRAD> int distill_launch(const Distill &a, hipStream_t s)
@@ -558,7 +565,7 @@ int distill_call(const char *fn, const dpx_array_view *logits, const dpx_array_v
     if (a.v > 0x3fffffff) return fail(DPX_ERR_BAD_ARGUMENT, f + "the last axis of logits is too long");
     if (k > MAX_K) return fail(DPX_ERR_BAD_ARGUMENT, f + "at most " + std::to_string(MAX_K) + " teacher entries per row");
     if (a.map.rows == 0) return DPX_OK;
-    const DistillPlan pl = distill_plan(a.map.rows, a.v, dt == DPX_DOUBLE);
+    const DistillPlan pl = distill_plan(a.map.rows, a.v, dt == DPX_DOUBLE, grad);
     if (a.map.rows * (pl.splits + 1) > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, f + "too many rows for one launch");
     const size_t need = (size_t)distill_workspace(logits, k);
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
