@@ -415,13 +415,13 @@ struct Workspace {
         bytes = (size_t)n;
     }
 };
-// Whether a kernel may write `out` although it reads `reads` (arrays or None): none overlaps it, but for those of `replaces`
+// Whether a kernel may write `out` although it reads `reads` (arrays, None or numbers): none overlaps it, but for those of `replaces`
 // that are the same array, element for element.
 bool may_write(py::handle out, py::tuple reads, py::tuple replaces)
 {
     dpx_array_view *vo = view_arg(out, "out");
     for (py::handle r : reads) {
-        if (r.is_none()) continue;
+        if (r.is_none() || PyFloat_CheckExact(r.ptr())) continue;
         dpx_array_view *vr = view_arg(r, "operand");
         if (!dpx_array_overlap(vr, vo)) continue;
         bool same = false;

@@ -47,18 +47,23 @@ def _vector(a, name):
     return _unit(a) if a._shape else a
 
 
-def _over_rows(a, lead, name, last=True):
-    """A side array seen with the rows `lead`: broadcast over them where it lacks them."""
+def _over_rows(a, lead, name):
+    """A side array with a last axis, seen with the rows `lead`: broadcast over them where it lacks them."""
     if a is None:
         return None
-    _array(a, name)
-    if last:
-        if not a._shape:
-            raise ValueError(f"{name} needs at least one dimension")
-        if a._shape[:-1] != lead:
-            a = broadcast_to(a, lead + a._shape[-1:])
-        return _unit(a)
-    return a if a._shape == lead else broadcast_to(a, lead)
+    shape = _array(a, name)._shape
+    if not shape:
+        raise ValueError(f"{name} needs at least one dimension")
+    if shape[:-1] != lead:
+        a = broadcast_to(a, lead + shape[-1:])
+    return a if a._strides[-1] == 1 else _unit(a)
+
+
+def _per_row(a, lead, name):
+    """A side array of one value per row."""
+    if a is None:
+        return None
+    return a if _array(a, name)._shape == lead else broadcast_to(a, lead)
 
 
 class _Out:
@@ -183,7 +188,7 @@ def distill_topk_grad(logits, teacher_logits, teacher_tokens, weights=None, /, *
     logits = _data(logits, "distill_topk_grad", "logits")
     lead = logits._shape[:-1]
     t, i = _over_rows(teacher_logits, lead, "teacher_logits"), _over_rows(teacher_tokens, lead, "teacher_tokens")
-    w = _over_rows(weights, lead, "weights", last=False)
+    w = _per_row(weights, lead, "weights")
     ol, od = _several(out, 2, "(loss, dlogits)")
     reads = (logits, t, i, w)
     loss = _Out(ol, lead, _acc(logits._dtype), "loss", reads)
@@ -194,11 +199,13 @@ def distill_topk_grad(logits, teacher_logits, teacher_tokens, weights=None, /, *
 
 
 def _penalty(p, lead, name, none):
+    if type(p) is usm_ndarray and p._shape == lead:
+        return p
     if p is None:
         return none
     if isinstance(p, numbers.Real):
         return float(p)
-    return _over_rows(p, lead, name, last=False)
+    return _per_row(p, lead, name)
 
 
 def process_logits(logits, /, *, prompt_tokens=None, prompt_lengths=None, output_tokens=None, output_lengths=None,
@@ -221,14 +228,13 @@ def process_logits(logits, /, *, prompt_tokens=None, prompt_lengths=None, output
     z = _data(logits, "process_logits", "logits")
     lead = z._shape[:-1]
     pt, ot = _over_rows(prompt_tokens, lead, "prompt_tokens"), _over_rows(output_tokens, lead, "output_tokens")
-    pl = _over_rows(prompt_lengths, lead, "prompt_lengths", last=False)
-    ol = _over_rows(output_lengths, lead, "output_lengths", last=False)
+    pl = _per_row(prompt_lengths, lead, "prompt_lengths")
+    ol = _per_row(output_lengths, lead, "output_lengths")
     rep = _penalty(repetition_penalty, lead, "repetition_penalty", 1.0)
     freq = _penalty(frequency_penalty, lead, "frequency_penalty", 0.0)
     pres = _penalty(presence_penalty, lead, "presence_penalty", 0.0)
     bt, bv = _over_rows(bias_tokens, lead, "bias_tokens"), _over_rows(bias_values, lead, "bias_values")
     ok = _over_rows(allowed, lead, "allowed")
-    reads = () if out is None else tuple(a for a in (z, pt, pl, ot, ol, rep, freq, pres, bt, bv, ok) if type(a) is not float)
-    res = _Out(out, z._shape, z._dtype, "out", reads, (z,))
+    res = _Out(out, z._shape, z._dtype, "out", (z, pt, pl, ot, ol, rep, freq, pres, bt, bv, ok), (z,))
     _ext.process_logits(z, pt, pl, ot, ol, rep, freq, pres, bt, bv, ok, res.kernel)
     return res.done()
