@@ -72,7 +72,9 @@ def test_layer_norm_refusals():
 
 
 def test_layer_norm_grad_refusals():
-    x, dy, dx, m, s, w = view((4, 8)), view((4, 8)), view((4, 8)), view((4,)), view((4,)), view((8,))
+    # (so many rows that the parameters' gradients need a workspace; few need none)
+    R = 400
+    x, dy, dx, m, s, w = view((R, 8)), view((R, 8)), view((R, 8)), view((R,)), view((R,)), view((8,))
     dw, db = view((8,)), view((8,))
     ws = ctypes.c_void_p(BASE)
     n = lib.dpx_layer_norm_grad_workspace(x)
@@ -80,22 +82,22 @@ def test_layer_norm_grad_refusals():
     def call(dy=dy, x=x, m=m, s=s, w=w, dx=dx, dw=dw, db=db, ws=ws, n=n):
         return lib.dpx_layer_norm_grad(dy, x, m, s, w, dx, dw, db, ws, n, None)
 
-    assert n > 0 and lib.dpx_layer_norm_grad_workspace(view((0, 8))) == 0
+    assert n > 0 and lib.dpx_layer_norm_grad_workspace(view((0, 8))) == lib.dpx_layer_norm_grad_workspace(view((4, 8))) == 0
     refused(call(n=n - 1), L.ERR_BAD_ARGUMENT, "workspace")
     refused(call(ws=None), L.ERR_BAD_ARGUMENT, "workspace")
     refused(call(ws=ctypes.c_void_p(BASE + 8)), L.ERR_BAD_ARGUMENT, "aligned")
     refused(call(db=None), L.ERR_BAD_ARGUMENT, "together")
     refused(call(dx=None), L.ERR_BAD_ARGUMENT, "needed")
     refused(call(m=None), L.ERR_BAD_ARGUMENT, "needed")
-    refused(call(dy=view((4, 8), L.HALF)), L.ERR_NOT_IMPLEMENTED, "float16")
+    refused(call(dy=view((R, 8), L.HALF)), L.ERR_NOT_IMPLEMENTED, "float16")
     refused(call(dy=view((3, 8))), L.ERR_SHAPE_MISMATCH, "leading")
-    refused(call(m=view((4, 1))), L.ERR_RANK_MISMATCH, "dimensions")
+    refused(call(m=view((R, 1))), L.ERR_RANK_MISMATCH, "dimensions")
     refused(call(dw=view((8,), L.HALF)), L.ERR_BAD_DTYPE, "type of weight")
     refused(call(dw=view((9,))), L.ERR_SHAPE_MISMATCH, "length 9")
     refused(call(dw=w), L.ERR_OVERLAP, "overlap")
     refused(call(db=dw), L.ERR_OVERLAP, "overlap")
-    refused(call(dx=view((4, 8), ptr=w.data)), L.ERR_OVERLAP, "overlap")
-    refused(call(dx=view((4, 8), ptr=x.data + 4)), L.ERR_OVERLAP, "overlap")
+    refused(call(dx=view((R, 8), ptr=w.data)), L.ERR_OVERLAP, "overlap")
+    refused(call(dx=view((R, 8), ptr=x.data + 4)), L.ERR_OVERLAP, "overlap")
     refused(call(dw=view((8,), ptr=dy.data)), L.ERR_OVERLAP, "overlap")
     refused(call(w=view((8,), L.DOUBLE), dw=view((8,), L.DOUBLE), db=view((8,), L.DOUBLE)), L.ERR_NOT_IMPLEMENTED, "float64")
 

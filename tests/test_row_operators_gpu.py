@@ -70,6 +70,23 @@ def test_layer_norm_lengths(n, dt, wdt):
     check_norm_grad(rng, x, w, mean, rstd)
 
 
+@pytest.mark.parametrize("dt,wdt", TYPES)
+@pytest.mark.parametrize("n", LENGTHS)
+def test_layer_norm_grad_of_more_rows(n, dt, wdt):
+    # around the number of rows up to which the parameters' gradients need no second launch, and in place, which needs it
+    rng = np.random.default_rng(n)
+    x, w, b = norm_data(rng, (130, n), dt, wdt)
+    _, mean, rstd = dpt.layer_norm(dev(x), dev(w), dev(b), stats=True)
+    for r in (127, 128, 129, 130) if n < 600 else (129,):
+        check_norm_grad(rng, x[:r], w, mean[:r], rstd[:r])
+    dy = rng.standard_normal((3, n)).astype(dt)
+    want = dpt.layer_norm_grad(dev(dy), dev(x[:3]), mean[:3], rstd[:3], dev(w))
+    for which in (0, 1):
+        dyd, xd = dev(dy), dev(x[:3])
+        got = check_norm_grad(rng, x[:3], w, mean[:3], rstd[:3], xd=xd, dyd=dyd, dy=dy, out=((dyd, xd)[which], None, None))
+        assert got[0] is (dyd, xd)[which] and np.array_equal(host(got[0]), host(want[0]))
+
+
 @pytest.mark.parametrize("dt,wdt", [("f2", "f4"), ("f4", "f4"), ("f8", "f8")])
 @pytest.mark.parametrize("shape", [(1, 1024), (1000, 8), (4097, 24), (2049, 100), (3001, 129), (1030, 1000), (700, 2056), (530, 4104),
                                    (259, 8200), (3, 5, 7, 64), (16, 0), (0, 16), (2, 0, 3)])
