@@ -15,9 +15,9 @@
 // what does not fit is read again while it is still in a cache.  Few long rows are split over blocks that leave (M, s) in the
 // caller's workspace, and a second launch joins them.
 //
-// Measured (rocprofv3): gradient of 2048 x 65536 float16 102 us (5.3 TB/s; its exponentials and the rest of its arithmetic
+// Measured (rocprofv3): gradient of 2048 x 65536 float16 101 us (5.3 TB/s; its exponentials and the rest of its arithmetic
 // take about 50 us of it, which the loads and stores of the other block of the CU hide only in part), of 513 x 100003
-// float32 85 us (one row more than two rounds of the 256 CUs; 512 rows 76), loss of 2048 x 131072 float16 85 us (6.3 TB/s).
+// float32 82 us (one row more than two rounds of the 256 CUs; 512 rows 75), loss of 2048 x 131072 float16 85 us (6.3 TB/s).
 // Tried and not kept: rows that come in while the gradients of the row before go out (persistent blocks, a held pack's
 // registers reloaded after its last use: 160 us, the row's state no longer fits the registers); packs held in LDS as well
 // (158 us for 513 x 100003); a wave of its own for the teacher's side (a block of 9 waves leaves room for one a CU: 111 us).
@@ -526,8 +526,10 @@ template <class T, class TT, bool GRAD> int distill_launch(const Distill &a, hip
             else if (packs <= 8192) run(integral_constant<int, 512>{}, integral_constant<int, 16>{});
             else run(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
         }
+        // (2048 rows of 131072 float16: 85.2 us with 1024 threads, 87 with 512; 8 rows of 32768 float32: 5.2 and 5.6)
         else if (packs <= 1024) run(integral_constant<int, 256>{}, integral_constant<int, 0>{});
-        else run(integral_constant<int, 512>{}, integral_constant<int, 0>{});
+        else if (packs <= 4096) run(integral_constant<int, 512>{}, integral_constant<int, 0>{});
+        else run(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
     }
     else {
         hipLaunchKernelGGL((distill_split_kernel<T, TT, GRAD>), dim3((unsigned)(a.map.rows * (a.splits + 1))), dim3(DST_BLOCK), lds, s, a);
