@@ -319,23 +319,26 @@ __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_k
         if (tid == BT - 64) ((A *)a.loss)[a.map.template off<4>(row)] = loss;
     }
     if constexpr (GRAD) {
-        const bool zero = te.mass == 0 || w == 0;
+        const bool zero = __builtin_amdgcn_readfirstlane(te.mass == 0 || w == 0); // (the same in all threads)
         const A coef = (A)a.temp * w, f = coef * (te.mass / q.s);
-        auto grad = [&](T x) { return zero ? A(0) : f * pow2(fma1((A)x, c, -q.m)); };
         T *to = dz + run.head;
+        auto dense = [&](auto grad) {
 #pragma unroll
-        for (int j = 0; j < HELD; ++j) {
-            keep_whole(held[j]); // (or the sum's conversions to float are kept for this loop, two registers for one)
-            run.store(to, j * BT + tid, held[j], grad);
-        }
-        for (int i = HELD * BT + tid; i < run.packs; i += U * BT) {
-            pack<T, E> x[U];
+            for (int j = 0; j < HELD; ++j) {
+                keep_whole(held[j]); // (or the sum's conversions to float are kept for this loop, two registers for one)
+                run.store(to, j * BT + tid, held[j], grad);
+            }
+            for (int i = HELD * BT + tid; i < run.packs; i += U * BT) {
+                pack<T, E> x[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) x[u] = run.template load<true>(i + u * BT);
+                for (int u = 0; u < U; ++u) x[u] = run.template load<true>(i + u * BT);
 #pragma unroll
-            for (int u = 0; u < U; ++u) run.store(to, i + u * BT, x[u], grad);
-        }
-        run.store_rest(to, tid, rest, grad);
+                for (int u = 0; u < U; ++u) run.store(to, i + u * BT, x[u], grad);
+            }
+            run.store_rest(to, tid, rest, grad);
+        };
+        if (zero) dense([](T) { return A(0); });
+        else dense([&](T x) { return f * pow2(fma1((A)x, c, -q.m)); });
         __syncthreads();
         for (int k = tid; k < a.k; k += BT)
             if (token[k] >= 0)
