@@ -639,3 +639,66 @@ def test_results_that_share_memory_are_refused():
     wide = dpt.empty((6, 16), dtype="f4")
     with pytest.raises(ValueError, match="overlap"):
         dpt.distill_topk_grad(x, x[:, :2], dpt.zeros((6, 2), dtype="i4"), out=(wide[:, 2], wide[:, ::2]))
+
+
+def test_millions_of_short_rows():
+    rng = np.random.default_rng(12)
+    x, w, b = norm_data(rng, (2 ** 21 + 3, 5), "f4", "f4")
+    _, mean, rstd = check_norm(x, w, b)
+    dy = rng.standard_normal(x.shape).astype("f4")
+    dx, dw, db = dpt.layer_norm_grad(dev(dy), dev(x), mean, rstd, dev(w))
+    want, tol = ref.layer_norm_grad(dy, x, host(mean), host(rstd), w)[:3], ref.layer_norm_grad_tolerances(dy, x, host(mean), host(rstd), w)
+    for got, one, t in zip((dx, dw, db), want, tol):
+        within(got, one, t)
+    z, t, tok = distill_data(rng, 100003, 7, 3, "f4")
+    check_distill(z, t, tok)
+    z, d = logits_data(rng, 2003, 9, "f4")
+    check_logits(z, d)
+
+
+def test_logits_empty_and_very_long_lists():
+    rng = np.random.default_rng(14)
+    z = rng.standard_normal((3, 1009)).astype("f4")
+    none = dpt.empty((3, 0), dtype="i8")
+    out = dpt.process_logits(dev(z), prompt_tokens=none, output_tokens=none, repetition_penalty=2.0, frequency_penalty=1.0,
+                             bias_tokens=none, bias_values=dpt.empty((3, 0), dtype="f4"))
+    assert np.array_equal(host(out), z)
+    tok = rng.integers(-50, 1100, (3, 60001))
+    tok[:, ::7] += 2 ** 33  # far outside
+    lengths = np.array([60001, 0, 33333], "i4")
+    got = host(dpt.process_logits(dev(z), output_tokens=dev(tok), output_lengths=dev(lengths), frequency_penalty=0.5, presence_penalty=0.25))
+    for i in range(3):
+        here = tok[i, :lengths[i]]
+        said = np.bincount(here[(here >= 0) & (here < 1009)], minlength=1009)
+        # two products and differences in float32
+        tol = 2.0 ** -24 * (4 * 0.5 * said + 2 * np.abs(z[i]) + 1)
+        assert (np.abs(got[i] - (z[i].astype("f8") - 0.5 * said - 0.25 * (said > 0))) <= tol).all()
+        assert np.array_equal(got[i][said == 0], z[i][said == 0])
+
+
+def test_calls_from_two_threads():
+    import threading
+    rng = np.random.default_rng(15)
+    sets = []
+    for r, n in ((300, 700), (257, 1025)):
+        x, w, b = norm_data(rng, (r, n), "f4", "f4")
+        a = [dev(v) for v in (x, w, b, rng.standard_normal(x.shape).astype("f4"))]
+        z, t, tok = (dev(v) for v in distill_data(rng, 4, 100003, 12, "f4"))
+
+        def call(a=a, z=z, t=t, tok=tok):
+            y, mean, rstd = dpt.layer_norm(a[0], a[1], a[2], stats=True)
+            return (y, *dpt.layer_norm_grad(a[3], a[0], mean, rstd, a[1]), *dpt.distill_topk_grad(z, t, tok))
+
+        sets.append((call, [host(v) for v in call()]))
+    wrong = []
+
+    def many(call, want):
+        for _ in range(50):
+            wrong.extend(1 for g, k in zip(call(), want) if not np.array_equal(host(g), k))
+
+    threads = [threading.Thread(target=many, args=s) for s in sets]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
