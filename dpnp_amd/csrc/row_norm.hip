@@ -11,7 +11,7 @@
 //
 // Measured (rocprofv3): forward of 16384 x 4096 float16 with float32 parameters 47 us (5.7 TB/s; one block per row that
 // reads the weights anew 60 us, one wave per row 56), 20011 x 1001 float32 29.5 us (5.4 TB/s: rows off the 16-byte grid);
-// backward of 16384 x 4096 float16 78 us + 4.7 for the fold of the column sums (5.2 TB/s), 2049 x 10007 float32 53 + 6.5.
+// backward of 16384 x 4096 float16 79 us + 4.8 for the fold of the column sums (5.1 TB/s), 2049 x 10007 float32 53 + 6.5.
 // The backward's time does not change with the prefetch distance (0, 1, 2 rows), the threads per row (256 to 1024) or its
 // arithmetic (9 against 16 instructions per element): it is what three streams of persistent blocks reach here.
 #include "row_ops.hpp"
@@ -156,33 +156,64 @@ template <class T, class W, int E, int PPL, int G, int BT> __global__ __launch_b
 }
 
 // Rows too long for a block's registers: blocks of 1024 threads walk down the rows and read each three times (the second
-// and third time from the memory-side cache), elements BT apart.
+// and third time from a cache; 1428 x 70000 float16 113 us, element by element 334).  f(base, skip) for the thread's packs of a row; as in PackAt the last one is moved back.  Only its own
+// elements are stored: a row may be worked on in place.
+template <int E, int BT, class F> DPX_D void each_pack(int64_t n, F f)
+{
+#pragma unroll 4
+    for (int64_t at = (int64_t)threadIdx.x * E; at < n; at += (int64_t)BT * E) {
+        const int64_t base = at + E <= n ? at : n - E;
+        f(base, (int)(at - base));
+    }
+}
+template <int E, class T, class A> DPX_D void store_own(T *p, int skip, const A (&o)[E])
+{
+    if (skip == 0) store_vals<E, true>(p, o);
+    else
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (e >= skip) p[e] = (T)o[e];
+}
 template <class T, class W, int BT> __global__ __launch_bounds__(BT) void norm_fwd_long_kernel(NormFwd a)
 {
     using A = acc_of<T>;
+    constexpr int E = 16 / (int)sizeof(T);
     __shared__ SumPart<1, A> lds[4][BT / 16];
     const int64_t n = a.n;
     int slot = 0;
     for (int64_t row = blockIdx.x; row < a.map.rows; row += gridDim.x, slot ^= 2) {
         const T *x = (const T *)a.x + a.map.template off<0>(row);
         A s[1] = {0};
-        for (int64_t i = threadIdx.x; i < n; i += BT) s[0] += (A)x[i];
+        each_pack<E, BT>(n, [&](int64_t at, int skip) {
+            const pack<T, E> v = load_pack<T, E, false>(x + at);
+#pragma unroll
+            for (int e = 0; e < E; ++e) s[0] += e >= skip ? (A)v.v[e] : A(0);
+        });
         row_sums<BT, BT>(s, lds, slot);
         const A mean = s[0] / (A)n;
         s[0] = 0;
-        for (int64_t i = threadIdx.x; i < n; i += BT) {
-            const A d = (A)x[i] - mean;
-            s[0] += d * d;
-        }
+        each_pack<E, BT>(n, [&](int64_t at, int skip) {
+            const pack<T, E> v = load_pack<T, E, false>(x + at);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const A d = e >= skip ? (A)v.v[e] - mean : A(0);
+                s[0] = row_fma(d, d, s[0]);
+            }
+        });
         row_sums<BT, BT>(s, lds, slot + 1);
         const A rstd = A(1) / row_sqrt(s[0] / (A)n + (A)a.eps);
         T *y = (T *)a.y + a.map.template off<1>(row);
-        for (int64_t i = threadIdx.x; i < n; i += BT) {
-            A o = ((A)x[i] - mean) * rstd;
-            if (a.w) o *= (A)((const W *)a.w)[i];
-            if (a.b) o += (A)((const W *)a.b)[i];
-            y[i] = (T)o;
-        }
+        each_pack<E, BT>(n, [&](int64_t at, int skip) {
+            const pack<T, E> v = load_pack<T, E>(x + at);
+            A w[E], b[E], o[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = 1, b[e] = 0;
+            if (a.w) load_vals<E, false>((const W *)a.w + at, w);
+            if (a.b) load_vals<E, false>((const W *)a.b + at, b);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = row_fma(((A)v.v[e] - mean) * rstd, w[e], b[e]);
+            store_own<E>(y + at, skip, o);
+        });
         if (threadIdx.x == 0) {
             if (a.mean) ((A *)a.mean)[a.map.template off<2>(row)] = mean;
             if (a.rstd) ((A *)a.rstd)[a.map.template off<3>(row)] = rstd;
@@ -361,36 +392,99 @@ __global__ __launch_bounds__(BT, OCC) void norm_grad_kernel(NormBwd a)
     }
 }
 
-// Rows too long for registers: two passes over the row, the sums for dw and db kept in the block's slice of the workspace
-// (each thread adds to its own elements of it).
+// Rows too long for registers.  dx: two passes over a row, the second from a cache.
 template <class T, class W, int BT> __global__ __launch_bounds__(BT) void norm_grad_long_kernel(NormBwd a)
 {
     using A = acc_of<T>;
+    constexpr int E = 16 / (int)sizeof(T);
     __shared__ SumPart<2, A> lds[2][BT / 16];
     const int64_t n = a.n;
-    A *part = a.part ? (A *)a.part + (int64_t)blockIdx.x * 2 * n : nullptr;
     int slot = 0;
     for (int64_t row = blockIdx.x; row < a.map.rows; row += gridDim.x, slot ^= 1) {
         const T *dy = (const T *)a.dy + a.map.template off<0>(row), *x = (const T *)a.x + a.map.template off<1>(row);
         const A mean = ((const A *)a.mean)[a.map.template off<3>(row)], rstd = ((const A *)a.rstd)[a.map.template off<4>(row)];
-        const bool first = row == (int64_t)blockIdx.x;
+        // h and g of a pack
+        auto both = [&](int64_t at, A(&h)[E], A(&g)[E]) {
+            const pack<T, E> vx = load_pack<T, E, false>(x + at), vd = load_pack<T, E, false>(dy + at);
+            A w[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = 1;
+            if (a.w) load_vals<E, false>((const W *)a.w + at, w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) h[e] = ((A)vx.v[e] - mean) * rstd, g[e] = (A)vd.v[e] * w[e];
+        };
         A s[2] = {0, 0};
-        for (int64_t i = threadIdx.x; i < n; i += BT) {
-            const A h = ((A)x[i] - mean) * rstd, d = (A)dy[i], g = a.w ? d * (A)((const W *)a.w)[i] : d;
-            s[0] += g;
-            s[1] += g * h;
-            if (part) {
-                part[i] = first ? d * h : part[i] + d * h;
-                part[n + i] = first ? d : part[n + i] + d;
-            }
-        }
+        each_pack<E, BT>(n, [&](int64_t at, int skip) {
+            A h[E], g[E];
+            both(at, h, g);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e >= skip) {
+                    s[0] += g[e];
+                    s[1] = row_fma(g[e], h[e], s[1]);
+                }
+        });
         row_sums<BT, BT>(s, lds, slot);
         const A c1 = s[0] / (A)n, c2 = s[1] / (A)n;
         T *dx = (T *)a.dx + a.map.template off<2>(row);
-        for (int64_t i = threadIdx.x; i < n; i += BT) {
-            const A h = ((A)x[i] - mean) * rstd, d = (A)dy[i], g = a.w ? d * (A)((const W *)a.w)[i] : d;
-            dx[i] = (T)((g - c1 - h * c2) * rstd);
+        each_pack<E, BT>(n, [&](int64_t at, int skip) {
+            A h[E], g[E], o[E];
+            both(at, h, g);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = row_fma(-h[e], c2, g[e] - c1) * rstd;
+            store_own<E>(dx + at, skip, o);
+        });
+    }
+}
+// dw and db of such rows: a second reading, by columns and in a launch before that of dx.  A lane per pack, the block's waves share
+// the rows of its split, whose sums go to a slice of the workspace.  (The sums kept in the workspace by the blocks that walk
+// down the rows: 842 us a call for 3051 x 32768 float16 instead of 227, 302 for 1525 x 16384 float64 instead of 216.)
+template <class T, int BT> __global__ __launch_bounds__(BT) void norm_grad_split_kernel(NormBwd a, int splits)
+{
+    using A = acc_of<T>;
+    constexpr int E = 16 / (int)sizeof(T), NW = BT / 64, U = 4;
+    __shared__ A lds[NW][2][E][64];
+    const int64_t n = a.n;
+    const uint32_t strips = (uint32_t)((n + 64 * E - 1) / (64 * E)), split = blockIdx.x / strips;
+    const int64_t left = (int64_t)(blockIdx.x - split * strips) * 64 * E;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int begin = (int)(a.map.rows * split / splits), end = (int)(a.map.rows * (split + 1) / splits);
+    auto base_of = [&](int l) { return left + (int64_t)l * E + E <= n ? left + (int64_t)l * E : n - E; };
+    const int64_t at = base_of(lane);
+    A dw[E], db[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) dw[e] = db[e] = 0;
+    for (int row = begin + wave; row < end; row += NW * U) {
+        pack<T, E> d[U], x[U];
+        A mean[U], rstd[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = row + u * NW < end ? row + u * NW : end - 1;
+            d[u] = load_pack<T, E, false>((const T *)a.dy + a.map.template off<0>(r) + at);
+            x[u] = load_pack<T, E, false>((const T *)a.x + a.map.template off<1>(r) + at);
+            mean[u] = ((const A *)a.mean)[a.map.template off<3>(r)];
+            rstd[u] = ((const A *)a.rstd)[a.map.template off<4>(r)];
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (row + u * NW < end)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    dw[e] = row_fma((A)d[u].v[e], ((A)x[u].v[e] - mean[u]) * rstd[u], dw[e]);
+                    db[e] += (A)d[u].v[e];
+                }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) lds[wave][0][e][lane] = dw[e], lds[wave][1][e][lane] = db[e];
+    __syncthreads();
+    A *part = (A *)a.part + (int64_t)split * 2 * n;
+    for (int i = threadIdx.x; i < 2 * E * 64; i += BT) {
+        const int l = i % 64, e = i / 64 % E, which = i / (64 * E);
+        A s = lds[0][which][e][l];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) s += lds[k][which][e][l];
+        const int64_t base = base_of(l);
+        if (e >= left + (int64_t)l * E - base) part[which * n + base + e] = s; // (elements moved back belong to the lane before)
     }
 }
 
@@ -525,7 +619,7 @@ template <class T> GradShape grad_shape(int64_t n)
     if (p <= 1024) return E == 4 ? GradShape{E, 512, 2, 512, 2} : GradShape{E, 1024, 1, 1024, 1};
     const int64_t ppl = (p + 511) / 512;
     if (ppl <= (E == 8 ? 4 : 8)) return {E, 512, (int)ppl, 512, 1};
-    return {0, 0, 0, 1024, 1};
+    return {0, 0, 0, 1024, 2};
 }
 template <int E, class F> bool grad_dispatch(const GradShape &s, F &&f)
 {
@@ -575,6 +669,15 @@ template <class T> int64_t norm_grad_blocks(int64_t rows, int64_t n)
 constexpr int64_t FEW_ROWS = 128;
 template <class T> bool norm_grad_columned(int64_t rows, int64_t n) { return rows > 0 && rows <= FEW_ROWS && grad_shape<T>(n).g; }
 
+// slices of the workspace that a fold adds up
+template <class T> int64_t norm_grad_parts(int64_t rows, int64_t n)
+{
+    if (rows == 0 || norm_grad_columned<T>(rows, n)) return 0;
+    if (grad_shape<T>(n).g) return norm_grad_blocks<T>(rows, n);
+    const int64_t strips = (n * (int64_t)sizeof(T) + 1023) / 1024; // four blocks a CU, 16 rows or more in each
+    return std::max<int64_t>(1, std::min((device_cus() * 4 + strips - 1) / strips, rows / 16));
+}
+
 template <class T, class W> int norm_grad_launch(NormBwd &a, hipStream_t s)
 {
     using A = acc_of<T>;
@@ -582,6 +685,7 @@ template <class T, class W> int norm_grad_launch(NormBwd &a, hipStream_t s)
     const int64_t blocks = norm_grad_blocks<T>(a.map.rows, a.n);
     const GradShape sh = grad_shape<T>(a.n);
     const bool columns = a.dw && norm_grad_columned<T>(a.map.rows, a.n);
+    const int64_t parts = norm_grad_parts<T>(a.map.rows, a.n);
     if (blocks > 0) {
         auto run = [&](auto e, auto ppl, auto g, auto bt, auto occ, auto ahead) {
             const size_t lds = (a.part && sh.g < sh.bt) ? (size_t)(2 * a.n) * sizeof(A) : 0;
@@ -596,14 +700,20 @@ template <class T, class W> int norm_grad_launch(NormBwd &a, hipStream_t s)
             if (columns && in_place) launch(0, column_blocks);
             launch(blocks, in_place ? 0 : column_blocks);
         };
-        if (!grad_dispatch<E>(sh, run))
+        if (!grad_dispatch<E>(sh, run)) {
+            if (a.dw) {
+                const int64_t strips = (a.n + 64 * E - 1) / (64 * E);
+                if (strips * parts > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, "layer_norm_grad: rows too long");
+                hipLaunchKernelGGL((norm_grad_split_kernel<T, 256>), dim3((unsigned)(strips * parts)), dim3(256), 0, s, a, (int)parts);
+            }
             hipLaunchKernelGGL((norm_grad_long_kernel<T, W, 1024>), dim3((unsigned)blocks), dim3(1024), 0, s, a);
+        }
     }
     if (a.dw && !columns) {
         const int64_t fold = (2 * a.n + FOLD_COLS - 1) / FOLD_COLS;
         if (fold > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, "layer_norm_grad: rows too long");
         hipLaunchKernelGGL((norm_grad_fold_kernel<W, A>), dim3((unsigned)fold), dim3(FOLD_COLS * FOLD_ROWS), 0, s, (const A *)a.part,
-                           blocks, a.n, (W *)a.dw, (W *)a.db);
+                           parts, a.n, (W *)a.dw, (W *)a.db);
     }
     const hipError_t rc = hipGetLastError();
     return rc == hipSuccess ? DPX_OK : fail_hip(rc, "layer_norm_grad launch");
@@ -655,16 +765,14 @@ int layer_norm_call(const dpx_array_view *x, const dpx_array_view *weight, const
     });
 }
 
-// blocks that leave partial sums for a fold
-template <class T> int64_t grad_parts(int64_t rows, int64_t n) { return norm_grad_columned<T>(rows, n) ? 0 : norm_grad_blocks<T>(rows, n); }
 int64_t grad_workspace(const dpx_array_view *x)
 {
     if (!view_ok(x) || x->nd < 1 || !row_float(x->dtype)) return 0;
     const int64_t n = last_extent(x);
     if (n == 0) return 0;
-    const int64_t rows = view_size(x) / n, parts = x->dtype == DPX_HALF    ? grad_parts<half_t>(rows, n)
-                                                   : x->dtype == DPX_FLOAT ? grad_parts<float>(rows, n)
-                                                                           : grad_parts<double>(rows, n);
+    const int64_t rows = view_size(x) / n, parts = x->dtype == DPX_HALF    ? norm_grad_parts<half_t>(rows, n)
+                                                   : x->dtype == DPX_FLOAT ? norm_grad_parts<float>(rows, n)
+                                                                           : norm_grad_parts<double>(rows, n);
     return parts * 2 * n * itemsize_of(acc_dtype(x->dtype));
 }
 
