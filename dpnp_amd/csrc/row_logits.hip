@@ -126,9 +126,10 @@ template <class T, int E> DPX_D void keep_allowed(pack<T, E> &x, uint32_t bits)
     x = u.p;
 }
 
-// A block takes a run of a row's steps, CHUNK neighbouring tokens at a time, the next chunk's logits on their way.  Per chunk the lists' tokens are counted in LDS words; then every thread looks at the words of its own packs, and
-// where there are any, puts the pack into its place in LDS and processes the named tokens there one by one (a wave runs as
-// many rounds as the most named pack of its lanes has, mostly one), clears the words, and stores the pack.
+// A block takes a run of a row's steps, CHUNK neighbouring tokens at a time, the next chunk's logits on their way.  Per chunk
+// the lists' tokens are counted in LDS words; then every thread looks at the words of its own packs, and where there are any,
+// puts the pack into its place in LDS and processes the named tokens there one by one (a wave runs as many rounds as the most
+// named pack of its lanes has, mostly one), clears the words, and stores the pack.
 template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void logits_kernel(Logits a)
 {
     using A = acc_of<T>;

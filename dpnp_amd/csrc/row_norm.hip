@@ -155,9 +155,10 @@ template <class T, class W, int E, int PPL, int G, int BT> __global__ __launch_b
     }
 }
 
-// Rows too long for a block's registers: blocks of 1024 threads walk down the rows and read each three times (the second
-// and third time from a cache; 1428 x 70000 float16 113 us, element by element 334).  f(base, skip) for the thread's packs of a row; as in PackAt the last one is moved back.  Only its own
-// elements are stored: a row may be worked on in place.
+// Rows too long for a block's registers: blocks of 1024 threads walk down the rows and read each three times (the second and
+// third time from a cache; 1428 x 70000 float16 113 us, element by element 334).
+// f(base, skip) for the thread's packs of a row; as in PackAt the last one is moved back.  Only its own elements are stored: a
+// row may be worked on in place.
 template <int E, int BT, class F> DPX_D void each_pack(int64_t n, F f)
 {
 #pragma unroll 4
