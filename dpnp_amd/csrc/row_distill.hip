@@ -5,14 +5,18 @@
 //   loss = T^2 sum_k p_k (log p_k - log q[i_k])            (a term with p_k = 0 is 0; no entries: the loss is 0)
 //   d loss / d z[v] = T (q[v] P - sum over k with i_k = v of p_k),   P = sum_k p_k: 1, or 0 where no entry is there
 //
-// The vocabulary is what costs: the loss reads V logits, the gradient reads and writes V.  Exponentials are taken to base 2:
-// e_v = 2^(z_v c - M) with c = log2(e) / T, M = c max(z) rounded, as one fused multiply-add and one exponential instruction.
-// M's rounding multiplies every e_v of the row by the same factor, which the sum s = sum e_v takes out again (log q_v =
-// (z_v c - M) ln 2 - ln s, with the same M), so a common offset of the logits costs no accuracy.  Statistics and sums are
-// float32 (float64 for float64 logits).
+// The vocabulary is what costs: the loss reads V logits, the gradient reads and writes V.  Exponentials are taken to base 2,
+// relative to the largest logit m as it is: e_v = 2^((z_v - m) c) with c = log2(e) / T, s = sum e_v.  A difference and a product per
+// logit; where |m c| is small (form NEAR) one fused multiply-add stands for both, z_v c - M with M = m c rounded, and the factor
+// 2^(m c - M) that M's rounding leaves on all of them is taken out of the sum and of the gradient's factor.  Beyond it that
+// factor, and then m c itself, leave the type's range, while the differences do not: rows of the type's lowest value have the
+// softmax that their differences give.  Statistics and sums are float32 (float64 for float64 logits).
+//
+// In the logits' own unit the loss is T sum p_k ((t_k - max t) - (z_k - m)) + T^2 P (ln s - ln s_t): a teacher's token that the
+// student has masked with the lowest value costs what it should and no infinity.
 //
 // A block owns a row.  Its logits are read once, HELD packs per thread stay in registers between the sum and the gradient,
-// what does not fit is read again while it is still in a cache.  Few long rows are split over blocks that leave (M, s) in the
+// what does not fit is read again while it is still in a cache.  Few long rows are split over blocks that leave (m, s) in the
 // caller's workspace, and a second launch joins them.
 //
 // Measured (rocprofv3): gradient of 2048 x 65536 float16 101 us (5.3 TB/s; its exponentials and the rest of its arithmetic
@@ -31,7 +35,7 @@ struct Distill {
     RowMap<6> map; // logits, teacher, tokens, weights, loss, dlogits
     const void *z, *t, *tok, *wt;
     void *loss, *dz;
-    void *part; // split rows: [rows][splits] pairs (M, s), then [rows][3 k + 2] values of the teacher's side
+    void *part; // split rows: [rows][splits] pairs (m, s), then [rows][3 k + 3] values of the teacher's side
     int64_t v, chunk;
     int32_t k, tok64, splits;
     int32_t table; // gradient: size of the token table
@@ -45,32 +49,46 @@ DPX_D double ln(double x) { return ::log(x); }
 DPX_D float fma1(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 DPX_D double fma1(double a, double b, double c) { return __builtin_fma(a, b, c); }
 template <class A> DPX_D A neg_inf() { return -(A)__builtin_inff(); }
-template <class A> DPX_D A scale_of(const Distill &a) { return (A)(1.4426950408889634074 / a.temp); }
+// (finite for the smallest temperatures too: 0 c is 0)
+template <class A> DPX_D A scale_of(const Distill &a)
+{
+    return (A)__builtin_fmin(1.4426950408889634074 / a.temp, sizeof(A) == 4 ? (double)__FLT_MAX__ : __DBL_MAX__);
+}
 
-// Largest scaled logit M and sum of 2^(z c - M).  While M is -inf (nothing but -inf so far) the exponentials are taken relative
+// Largest logit m and sum of 2^((z - m) c).  While m is -inf (nothing but -inf so far) the exponentials are taken relative
 // to 0, which leaves the sum at 0 and lets a NaN through; the maximum itself passes NaN over.
 template <class A> struct Soft {
     A m, s;
 };
 template <class A> DPX_D A anchor(A m) { return m == neg_inf<A>() ? A(0) : m; }
-template <class A> DPX_D Soft<A> soft_join(Soft<A> a, Soft<A> b)
+template <class A> DPX_D A far_exp(A x, A m, A c) { return pow2((x - m) * c); }
+// 2^(x c - M), M = m c rounded, takes the place of 2^((x - m) c) up to |M| = NEAR_LIMIT: float32's M is off by at most 1 there, so
+// the factor 2^(m c - M) between the two stays near 1.  near_factor is its inverse.
+// The form is chosen by the row for float32 (BY_ROW), by the temperature for float16, whose largest value is known (a choice by
+// the row takes 12 registers more there, which spill: gradient of 4096 x 16000 61 us, not 54); float64 is FAR always, where an
+// exponential takes some thirty instructions and one more does not count.
+enum Form { NEAR, FAR, BY_ROW };
+constexpr float NEAR_LIMIT = 1 << 24;
+template <class A> DPX_D bool is_near(A M) { return M >= -NEAR_LIMIT && M <= NEAR_LIMIT; }
+template <class A> DPX_D A near_factor(A m, A c, A M) { return pow2(-fma1(m, c, -M)); }
+template <class A> DPX_D Soft<A> soft_join(Soft<A> a, Soft<A> b, A c)
 {
     const A m = MaxOp{}(a.m, b.m), z = anchor(m);
-    return {m, a.s * pow2(a.m - z) + b.s * pow2(b.m - z)};
+    return {m, a.s * far_exp(a.m, z, c) + b.s * far_exp(b.m, z, c)};
 }
 // over G lanes, the result in all of them
-template <int G, class A> DPX_D Soft<A> soft_lanes(Soft<A> v)
+template <int G, class A> DPX_D Soft<A> soft_lanes(Soft<A> v, A c)
 {
     const A m = lanes_fold<G>(v.m, MaxOp{});
-    return {m, lanes_fold<G>(v.s * pow2(v.m - anchor(m)), SumOp{})};
+    return {m, lanes_fold<G>(v.s * far_exp(v.m, anchor(m), c), SumOp{})};
 }
 // over a block of up to 1024 threads, in two halves around a barrier of the caller's
-template <class A> DPX_D void soft_leave(Soft<A> v, Soft<A> *lds)
+template <class A> DPX_D void soft_leave(Soft<A> v, A c, Soft<A> *lds)
 {
-    v = soft_lanes<64>(v);
+    v = soft_lanes<64>(v, c);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
 }
-template <int BT, class A> DPX_D Soft<A> soft_collect(const Soft<A> *lds)
+template <int BT, class A> DPX_D Soft<A> soft_collect(const Soft<A> *lds, A c)
 {
     constexpr int NW = BT / 64;
     static_assert(NW == 2 || NW == 4 || NW == 8 || NW == 16);
@@ -78,7 +96,7 @@ template <int BT, class A> DPX_D Soft<A> soft_collect(const Soft<A> *lds)
     const int lane = threadIdx.x & 15;
     Soft<A> v = lds[lane & (NW - 1)];
     if (lane >= NW) v.s = 0;
-    return soft_lanes<16>(v);
+    return soft_lanes<16>(v, c);
 }
 
 template <class T, int E> DPX_D acc_of<T> pack_max(const pack<T, E> &v)
@@ -95,20 +113,28 @@ template <class T, int E> DPX_D pack<T, E> pack_max2(pack<T, E> a, const pack<T,
     for (int e = 0; e < E; ++e) a.v[e] = __builtin_elementwise_max(a.v[e], b.v[e]);
     return a;
 }
-// U packs joined into a running (M, s): one rescaling for all of them
-template <class T, int E, int U, class A> DPX_D void soft_take(Soft<A> &r, const pack<T, E> *x, A c)
+// U packs joined into a running (m, s): one rescaling for all of them
+template <Form FORM, class T, int E, int U, class A> DPX_D void soft_take(Soft<A> &r, const pack<T, E> *x, A c)
 {
     pack<T, E> top = x[0];
 #pragma unroll
     for (int u = 1; u < U; ++u) top = pack_max2(top, x[u]);
-    const A m = MaxOp{}(r.m, pack_max(top) * c), z = anchor(m);
-    A s[4] = {r.s * pow2(r.m - z), 0, 0, 0};
+    const A m = MaxOp{}(r.m, pack_max(top)), z = anchor(m), M = z * c;
+    A s[4] = {0, 0, 0, 0}, f = 1;
+    auto add = [&](auto exponential) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[(u * E + e) & 3] += pow2(fma1((A)x[u].v[e], c, -z));
+            for (int e = 0; e < E; ++e) s[(u * E + e) & 3] += exponential((A)x[u].v[e]);
+    };
+    // (a branch of the whole wave)
+    if (FORM == NEAR || (FORM == BY_ROW && __builtin_amdgcn_ballot_w64(!is_near(M)) == 0)) {
+        add([&](A v) { return pow2(fma1(v, c, -M)); });
+        f = near_factor(z, c, M);
+    }
+    else add([&](A v) { return far_exp(v, z, c); });
+    r.s = fma1((s[0] + s[1]) + (s[2] + s[3]), f, r.s * far_exp(r.m, z, c));
     r.m = m;
-    r.s = (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 // A run of n logits: packs that start on a 128-byte line, and the elements before them (fewer than LINE) and behind them
@@ -154,15 +180,16 @@ template <class T, int E> struct Run {
 };
 template <class T, class A> DPX_D Soft<A> soft_one(Soft<A> r, T x, A c) // one element more
 {
-    const A m = MaxOp{}(r.m, (A)x * c), z = anchor(m);
-    return {m, r.s * pow2(r.m - z) + pow2(fma1((A)x, c, -z))};
+    const A m = MaxOp{}(r.m, (A)x), z = anchor(m);
+    return {m, r.s * far_exp(r.m, z, c) + far_exp((A)x, z, c)};
 }
 
 // ---- the teacher's side of a row, by one wave -----------------------------------------------------------------------------
 // p[k] (0 where absent), the student's logit zk[k] at the entry's token and the token itself (-1 where absent); in `sum` the
-// mass sum(p) (1, 0 with no entry that counts, or NaN) and sum p ln p.
+// mass sum(p) (1, 0 with no entry that counts, or NaN), sum p (t - max t) / 2 and the logarithm of the entries' sum.
+// (Halves: the difference of two finite logits may not be finite.)
 template <class A> struct TeacherSum {
-    A mass, plogp;
+    A mass, half, lns;
     bool repeats; // some token belongs to several entries
 };
 // The row's tokens in a hash table in LDS (open addressing, at most a quarter full), which tells those of several entries:
@@ -232,30 +259,29 @@ DPX_D TeacherSum<A> teacher_wave(const Distill &a, int64_t row, A c, Entry<A> fi
         p[k] = x;
         if constexpr (GRAD)
             if (there) repeats |= table_put(table, a.table, (uint32_t)f.token);
-        const A m = MaxOp{}(s.m, x * c), anc = anchor(m);
-        s.s = s.s * pow2(s.m - anc) + pow2(fma1(x, c, -anc));
-        s.m = m;
+        s = soft_join(s, Soft<A>{x, 1}, c);
     }
-    s = soft_lanes<64>(s);
+    s = soft_lanes<64>(s, c);
     const bool none = s.m == neg_inf<A>() && s.s == 0;
-    const A inv = none ? A(0) : A(1) / s.s, m = anchor(s.m), lns = ln(s.s);
-    A plogp = 0;
+    const A inv = none ? A(0) : A(1) / s.s, m = anchor(s.m);
+    A half = 0;
     for (int k = lane; k < a.k; k += 64) {
-        const A e = fma1(p[k], c, -m), pk = none ? A(0) : pow2(e) * inv;
+        const A x = p[k], pk = none ? A(0) : far_exp(x, m, c) * inv;
         p[k] = pk;
-        if (pk != 0) plogp += pk * (e * (A)0.69314718055994530942 - lns);
+        if (pk != 0) half += pk * fma1(x, A(0.5), m * A(-0.5));
     }
-    return {none ? A(0) : s.s * inv, lanes_fold<64>(plogp, SumOp{}), __builtin_amdgcn_ballot_w64(repeats) != 0};
+    return {none ? A(0) : s.s * inv, lanes_fold<64>(half, SumOp{}), ln(s.s), __builtin_amdgcn_ballot_w64(repeats) != 0};
 }
-// loss of the row from the student's (M, s): by one wave
-template <class A> DPX_D A loss_wave(const Distill &a, Soft<A> q, TeacherSum<A> te, A c, const A *p, const A *zk)
+// loss of the row from the student's (m, s): by one wave
+template <class A> DPX_D A loss_wave(const Distill &a, Soft<A> q, TeacherSum<A> te, const A *p, const A *zk)
 {
-    const A lns = ln(q.s);
-    A sum = 0;
+    A half = 0;
     for (int k = threadIdx.x & 63; k < a.k; k += 64)
-        if (p[k] != 0) sum += p[k] * (fma1(zk[k], c, -q.m) * (A)0.69314718055994530942 - lns);
-    sum = lanes_fold<64>(sum, SumOp{});
-    return te.mass == 0 ? A(0) : (A)(a.temp * a.temp) * (te.plogp - sum);
+        if (p[k] != 0) half += p[k] * fma1(zk[k], A(0.5), q.m * A(-0.5));
+    half = lanes_fold<64>(half, SumOp{});
+    // (T^2 may be beyond float32 where the loss is not)
+    return te.mass == 0 ? A(0)
+                        : (A)(2 * a.temp * (double)(te.half - half) + a.temp * a.temp * (double)(te.mass * (ln(q.s) - te.lns)));
 }
 // all the weight that entry k's token gets, its own and that of other entries with the same token, in their order
 template <class A> DPX_D A token_weight(const Distill &a, bool repeats, const A *p, const int32_t *token, int k)
@@ -273,7 +299,7 @@ template <class A> DPX_D A token_weight(const Distill &a, bool repeats, const A 
 // the teacher's side, whose first entries are sent for before the row.  The gradient is stored densely first, a barrier, then
 // the values at the teacher's tokens over it (their logits were read at the start: dz may be z).  A row of weight 0, and
 // one without entries, gets zeros whatever its logits are.
-template <class T, class TT, int BT, int HELD, bool GRAD>
+template <class T, class TT, int BT, int HELD, bool GRAD, Form FORM>
 __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_kernel(Distill a)
 {
     using A = acc_of<T>;
@@ -303,32 +329,28 @@ __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_k
     const A w = GRAD ? (a.wt ? ((const A *)a.wt)[a.map.template off<3>(row)] : A(1)) : A(0);
     Soft<A> r = soft_one(Soft<A>{neg_inf<A>(), 0}, rest, c);
 #pragma unroll
-    for (int j = 0; j < HELD; j += U) soft_take<T, E, U>(r, held + j, c);
+    for (int j = 0; j < HELD; j += U) soft_take<FORM, T, E, U>(r, held + j, c);
     for (int q = HELD * BT + tid; q < run.packs; q += U * BT) {
         pack<T, E> x[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) x[u] = run.template load<!GRAD>(q + u * BT);
-        soft_take<T, E, U>(r, x, c);
+        soft_take<FORM, T, E, U>(r, x, c);
     }
-    soft_leave(r, waves);
+    soft_leave(r, c, waves);
     __syncthreads();
-    const Soft<A> q = soft_collect<BT>(waves);
+    const Soft<A> q = soft_collect<BT>(waves, c);
     const TeacherSum<A> te = teacher;
     if (tid >= BT - 64) {
-        const A loss = loss_wave(a, q, te, c, p, zk);
+        const A loss = loss_wave(a, q, te, p, zk);
         if (tid == BT - 64) ((A *)a.loss)[a.map.template off<4>(row)] = loss;
     }
     if constexpr (GRAD) {
         const bool zero = __builtin_amdgcn_readfirstlane(te.mass == 0 || w == 0); // (the same in all threads)
-        const A coef = (A)a.temp * w, f = coef * (te.mass / q.s);
+        const A coef = (A)a.temp * w, f = coef * (te.mass / q.s), M = q.m * c;
+        const bool near = FORM == NEAR || (FORM == BY_ROW && __builtin_amdgcn_readfirstlane(is_near(M)));
         T *to = dz + run.head;
-        auto dense = [&](auto grad) {
-#pragma unroll
-            for (int j = 0; j < HELD; ++j) {
-                keep_whole(held[j]); // (or the sum's conversions to float are kept for this loop, two registers for one)
-                run.store(to, j * BT + tid, held[j], grad);
-            }
-            for (int i = HELD * BT + tid; i < run.packs; i += U * BT) {
+        auto reread = [&](int i, auto grad) {
+            for (; i < run.packs; i += U * BT) {
                 pack<T, E> x[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) x[u] = run.template load<true>(i + u * BT);
@@ -337,25 +359,41 @@ __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_k
             }
             run.store_rest(to, tid, rest, grad);
         };
+        auto dense = [&](auto grad) {
+#pragma unroll
+            for (int j = 0; j < HELD; ++j) {
+                keep_whole(held[j]); // (or the sum's conversions to float are kept for this loop, two registers for one)
+                run.store(to, j * BT + tid, held[j], grad);
+            }
+            reread(HELD * BT + tid, grad);
+        };
         if (zero) dense([](T) { return A(0); });
-        else dense([&](T x) { return f * pow2(fma1((A)x, c, -q.m)); });
+        else if (near) {
+            const A g = f * near_factor(q.m, c, M);
+            dense([&](T x) { return g * pow2(fma1((A)x, c, -M)); });
+        }
+        else {
+            auto grad = [&](T x) { return f * far_exp((A)x, q.m, c); };
+            if constexpr (FORM == BY_ROW) reread(tid, grad); // (rare: the held packs are let go, which saves the registers)
+            else dense(grad);
+        }
         __syncthreads();
         for (int k = tid; k < a.k; k += BT)
             if (token[k] >= 0)
-                dz[token[k]] = (T)(zero ? A(0) : f * pow2(fma1(zk[k], c, -q.m)) - coef * token_weight(a, te.repeats, p, token, k));
+                dz[token[k]] = (T)(zero ? A(0) : f * far_exp(zk[k], q.m, c) - coef * token_weight(a, te.repeats, p, token, k));
     }
 }
 
 // ---- few long rows: split over blocks -------------------------------------------------------------------------------------------
 constexpr int DST_BLOCK = 256;
-// the teacher's side of a row in the workspace: mass, sum p ln p, then p, zk and the tokens' weights
+// the teacher's side of a row in the workspace: its TeacherSum, then p, zk and the tokens' weights
 template <class A> DPX_D A *teacher_part(const Distill &a, int64_t row)
 {
-    return (A *)a.part + a.map.rows * a.splits * 2 + row * (3 * (int64_t)a.k + 2);
+    return (A *)a.part + a.map.rows * a.splits * 2 + row * (3 * (int64_t)a.k + 3);
 }
 
-// first launch: block (row, split) leaves (M, s) of its part; the last split of a row the teacher's side
-template <class T, class TT, bool GRAD> __global__ __launch_bounds__(DST_BLOCK) void distill_split_kernel(Distill a)
+// first launch: block (row, split) leaves (m, s) of its part; the last split of a row the teacher's side
+template <class T, class TT, bool GRAD, Form FORM> __global__ __launch_bounds__(DST_BLOCK) void distill_split_kernel(Distill a)
 {
     using A = acc_of<T>;
     constexpr int E = 16 / (int)sizeof(T), U = 4;
@@ -373,15 +411,16 @@ template <class T, class TT, bool GRAD> __global__ __launch_bounds__(DST_BLOCK) 
             const TeacherSum<A> te = teacher_wave<T, TT, GRAD>(a, row, c, teacher_entry<T, TT, A>(a, row, tid), p, zk, token);
             if (tid == 0) {
                 to[0] = te.mass;
-                to[1] = te.plogp;
+                to[1] = te.half;
+                to[2] = te.lns;
                 repeats = te.repeats;
             }
         }
         __syncthreads();
         for (int k = tid; k < a.k; k += DST_BLOCK) {
-            to[2 + k] = p[k];
-            to[2 + a.k + k] = zk[k];
-            if constexpr (GRAD) to[2 + 2 * a.k + k] = token_weight(a, repeats, p, token, k);
+            to[3 + k] = p[k];
+            to[3 + a.k + k] = zk[k];
+            if constexpr (GRAD) to[3 + 2 * a.k + k] = token_weight(a, repeats, p, token, k);
         }
         return;
     }
@@ -393,21 +432,21 @@ template <class T, class TT, bool GRAD> __global__ __launch_bounds__(DST_BLOCK) 
         pack<T, E> x[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) x[u] = run.template load<false>(q + u * DST_BLOCK);
-        soft_take<T, E, U>(r, x, c);
+        soft_take<FORM, T, E, U>(r, x, c);
     }
-    soft_leave(r, waves);
+    soft_leave(r, c, waves);
     __syncthreads();
-    r = soft_collect<DST_BLOCK>(waves);
+    r = soft_collect<DST_BLOCK>(waves, c);
     if (tid == 0) ((Soft<A> *)a.part)[row * a.splits + split] = r;
 }
 
-// a row's (M, s) from its parts, the same in every lane: read by the 64 lanes of a wave, joined by DPP
-template <class A> DPX_D Soft<A> soft_row(const Distill &a, int64_t row)
+// a row's (m, s) from its parts, the same in every lane: read by the 64 lanes of a wave, joined by DPP
+template <class A> DPX_D Soft<A> soft_row(const Distill &a, int64_t row, A c)
 {
     const Soft<A> *p = (const Soft<A> *)a.part + row * a.splits;
     Soft<A> r{neg_inf<A>(), 0};
-    for (int k = threadIdx.x & 63; k < a.splits; k += 64) r = soft_join(r, p[k]);
-    return soft_lanes<64>(r);
+    for (int k = threadIdx.x & 63; k < a.splits; k += 64) r = soft_join(r, p[k], c);
+    return soft_lanes<64>(r, c);
 }
 
 // second launch: the loss, and with GRAD the gradient of block (row, split)'s part
@@ -422,10 +461,10 @@ template <class T, bool GRAD> __global__ __launch_bounds__(GRAD ? DST_BLOCK : 64
     const A *te = teacher_part<A>(a, row);
     auto loss = [&](Soft<A> q) {
         if (split != 0 || tid >= 64) return;
-        const A l = loss_wave(a, q, TeacherSum<A>{te[0], te[1], false}, c, te + 2, te + 2 + a.k);
+        const A l = loss_wave(a, q, TeacherSum<A>{te[0], te[1], te[2], false}, te + 3, te + 3 + a.k);
         if (tid == 0) ((A *)a.loss)[a.map.template off<4>(row)] = l;
     };
-    if constexpr (!GRAD) loss(soft_row<A>(a, row));
+    if constexpr (!GRAD) loss(soft_row<A>(a, row, c));
     else {
         // everything that does not wait for the row's sum is sent for before it
         const int begin = (int)(split * a.chunk), end = (int)(begin + a.chunk < a.v ? begin + a.chunk : a.v), n = end - begin;
@@ -444,14 +483,14 @@ template <class T, bool GRAD> __global__ __launch_bounds__(GRAD ? DST_BLOCK : 64
         auto entry = [&](int k) {
             if (k >= a.k) return Named{-1, 0, 0};
             const int64_t token = a.tok64 ? ((const int64_t *)a.tok)[to + k] : (int64_t)((const int32_t *)a.tok)[to + k];
-            return Named{token - begin, te[2 + a.k + k], te[2 + 2 * a.k + k]};
+            return Named{token - begin, te[3 + a.k + k], te[3 + 2 * a.k + k]};
         };
         const Named mine = entry(tid);
         const A w = a.wt ? ((const A *)a.wt)[a.map.template off<3>(row)] : A(1), mass = te[0];
-        const Soft<A> q = soft_row<A>(a, row);
+        const Soft<A> q = soft_row<A>(a, row, c);
         const bool zero = mass == 0 || w == 0;
         const A coef = (A)a.temp * w, f = coef * (mass / q.s);
-        auto grad = [&](T x) { return zero ? A(0) : f * pow2(fma1((A)x, c, -q.m)); };
+        auto grad = [&](T x) { return zero ? A(0) : f * far_exp((A)x, q.m, c); };
         run.store_rest(first, tid, one, grad);
         for (int i = tid;;) {
 #pragma unroll
@@ -465,7 +504,7 @@ template <class T, bool GRAD> __global__ __launch_bounds__(GRAD ? DST_BLOCK : 64
         __syncthreads();
         for (int k = tid; k < a.k; k += DST_BLOCK) {
             const Named t = k < DST_BLOCK ? mine : entry(k);
-            if (t.at >= 0 && t.at < n) dz[t.at] = (T)(zero ? A(0) : f * pow2(fma1(t.z, c, -q.m)) - coef * t.weight);
+            if (t.at >= 0 && t.at < n) dz[t.at] = (T)(zero ? A(0) : f * far_exp(t.z, q.m, c) - coef * t.weight);
         }
     }
 }
@@ -506,10 +545,10 @@ int64_t distill_workspace(const dpx_array_view *z, int64_t k)
     if (rows == 0) return 0;
     const bool is_double = z->dtype == DPX_DOUBLE; // (one size for the loss alone and with its gradient)
     const int64_t splits = std::max(distill_plan(rows, v, is_double, false).splits, distill_plan(rows, v, is_double, true).splits);
-    return splits ? rows * (splits * 2 + 3 * k + 2) * itemsize_of(acc_dtype(z->dtype)) : 0;
+    return splits ? rows * (splits * 2 + 3 * k + 3) * itemsize_of(acc_dtype(z->dtype)) : 0;
 }
 
-template <class T, class TT, bool GRAD> int distill_launch(const Distill &a, hipStream_t s)
+template <class T, class TT, bool GRAD, Form FORM> int distill_launch(const Distill &a, hipStream_t s)
 {
     using A = acc_of<T>;
     constexpr int E = 16 / (int)sizeof(T);
@@ -519,9 +558,10 @@ template <class T, class TT, bool GRAD> int distill_launch(const Distill &a, hip
         const int64_t packs = (a.v + E - 1) / E;
         using std::integral_constant;
         auto run = [&](auto bt, auto held) {
-            hipLaunchKernelGGL((distill_row_kernel<T, TT, decltype(bt)::value, decltype(held)::value, GRAD>), rows, dim3(bt), lds, s, a);
+            hipLaunchKernelGGL((distill_row_kernel<T, TT, decltype(bt)::value, decltype(held)::value, GRAD, FORM>), rows, dim3(bt), lds, s, a);
         };
-        if constexpr (GRAD) {
+        if constexpr (FORM == FAR && sizeof(T) == 2) run(integral_constant<int, 512>{}, integral_constant<int, 0>{}); // (rare)
+        else if constexpr (GRAD) {
             if (packs <= 512) run(integral_constant<int, 128>{}, integral_constant<int, 4>{});
             else if (packs <= 1024) run(integral_constant<int, 256>{}, integral_constant<int, 4>{});
             else if (packs <= 2048) run(integral_constant<int, 256>{}, integral_constant<int, 8>{});
@@ -535,7 +575,7 @@ template <class T, class TT, bool GRAD> int distill_launch(const Distill &a, hip
         else run(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
     }
     else {
-        hipLaunchKernelGGL((distill_split_kernel<T, TT, GRAD>), dim3((unsigned)(a.map.rows * (a.splits + 1))), dim3(DST_BLOCK), lds, s, a);
+        hipLaunchKernelGGL((distill_split_kernel<T, TT, GRAD, FORM>), dim3((unsigned)(a.map.rows * (a.splits + 1))), dim3(DST_BLOCK), lds, s, a);
         if constexpr (GRAD) hipLaunchKernelGGL((distill_join_kernel<T, true>), dim3((unsigned)(a.map.rows * a.splits)), dim3(DST_BLOCK), 0, s, a);
         else hipLaunchKernelGGL((distill_join_kernel<T, false>), rows, dim3(64), 0, s, a);
     }
@@ -579,15 +619,21 @@ int distill_call(const char *fn, const dpx_array_view *logits, const dpx_array_v
     a.part = workspace;
     a.chunk = pl.chunk, a.splits = pl.splits, a.k = (int32_t)k, a.tok64 = tokens->dtype == DPX_INT64, a.temp = temperature;
     a.table = grad ? table_size((int)k) : 0;
-    auto run = [&](auto t, auto u) {
+    auto run = [&](auto t, auto u, auto form) {
         using T = typename decltype(t)::type;
         using TT = typename decltype(u)::type;
-        return grad ? distill_launch<T, TT, true>(a, stream) : distill_launch<T, TT, false>(a, stream);
+        return grad ? distill_launch<T, TT, true, decltype(form)::value>(a, stream)
+                    : distill_launch<T, TT, false, decltype(form)::value>(a, stream);
     };
-    if (dt == DPX_HALF && teacher->dtype == DPX_HALF) return run(tag<half_t>{}, tag<half_t>{});
-    if (dt == DPX_HALF) return run(tag<half_t>{}, tag<float>{});
-    if (dt == DPX_FLOAT) return run(tag<float>{}, tag<float>{});
-    return run(tag<double>{}, tag<double>{});
+    using std::integral_constant;
+    const integral_constant<Form, NEAR> near;
+    const integral_constant<Form, FAR> far;
+    if (dt == DPX_FLOAT) return run(tag<float>{}, tag<float>{}, integral_constant<Form, BY_ROW>{});
+    if (dt == DPX_DOUBLE) return run(tag<double>{}, tag<double>{}, far);
+    auto half = [&](auto u) {
+        return 65504 * 1.4426950408889634074 / temperature <= NEAR_LIMIT ? run(tag<half_t>{}, u, near) : run(tag<half_t>{}, u, far);
+    };
+    return teacher->dtype == DPX_HALF ? half(tag<half_t>{}) : half(tag<float>{});
 }
 
 } // namespace

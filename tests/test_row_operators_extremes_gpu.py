@@ -1,0 +1,178 @@
+"""The row operators at the ends of their ranges: values near the limits of a type, large offsets, calls larger than one
+launch, long lists."""
+import numpy as np
+import pytest
+
+import dpnp_amd.tensor as dpt
+from tests import row_operator_references as ref
+from tests.helpers import dev, host
+
+pytestmark = pytest.mark.gpu
+W = np.longdouble  # its exponents hold differences and products of float64's largest values
+
+
+def within(got, want, tol, what=""):
+    got = host(got)
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    with np.errstate(all="ignore"):
+        rounded = want.astype(got.dtype)  # (beyond the type's range: infinite)
+        bad = ~(np.abs(got.astype(W) - want) <= tol) & ~(np.isinf(rounded) & (got == rounded))
+    assert not bad.any(), (what, int(bad.sum()), np.argwhere(bad)[:3].tolist(), got[bad][:3], want[bad][:3],
+                           np.broadcast_to(tol, want.shape)[bad][:3])
+
+
+# ---- distillation --------------------------------------------------------------------------------------------------
+def distill(z, t, tok, temp, w):
+    """(loss, bound, gradient, bound) from the definition, in units of the logits so that nothing overflows.  The bounds count
+    the roundings as `distill_tolerances` does: three of an exponential's argument and 2 u of the function, a chain of
+    additions and rescalings of v / 128 + 64 at most per sum, and those of the final products."""
+    u = W(ref.unit(z.dtype))
+    dt, (r, v), k = z.dtype, z.shape, t.shape[1]
+    z, t, temp, w = z.astype(W), t.astype(W), W(temp), w.astype(W)
+    there = (tok >= 0) & (tok < v)
+    at = (np.arange(r)[:, None], np.where(there, tok, 0))
+    d = z - z.max(1)[:, None]
+    with np.errstate(under="ignore"):
+        e = np.exp(d / temp)
+    s = e.sum(1)[:, None]
+    q = e / s
+    some = there.any(1)[:, None]
+    top = np.where(there, t, -np.inf).max(1, initial=-np.inf)[:, None]
+    td = np.where(there, t - np.where(some, top, 0), 0)
+    with np.errstate(under="ignore"):
+        te = np.where(there, np.exp(td / temp), 0)
+    ts = np.where(some, te.sum(1)[:, None], 1)
+    p = te / ts
+    zk = d[at]
+    loss = np.where(p > 0, temp * p * (td - zk) + temp * temp * p * (np.log(s) - np.log(ts)), 0).sum(1)
+    grad = q * some
+    np.subtract.at(grad, at, p)
+    grad *= (temp * w)[:, None]
+    grad[w == 0] = 0
+    # bounds
+    de, dp = u * (3 * np.abs(d) / temp + 2), u * (3 * np.abs(td) / temp + 2)
+    ds = (q * de).sum(1)[:, None] + u * (W(v) / 128 + 64)
+    dps = (p * dp).sum(1)[:, None] + u * (W(k) / 64 + 32)
+    size = temp * (np.abs(td) + np.abs(zk)) + temp * temp * (np.log(s) + np.log(ts))
+    t_loss = (p * (dp + dps + u * (W(k) / 64 + 40)) * size + p * temp * temp * (ds + dps)).sum(1) * W(1.01) + W(1e-37)
+    sp = np.zeros_like(q)
+    np.add.at(sp, at, p * (dp + dps + (k + 4) * u))
+    t = np.abs(temp * w)[:, None] * (q * (de + ds + 8 * u) + sp) * W(1.01) + W(1e-37)
+    half = np.maximum((np.abs(grad) + t) * W(np.finfo(dt).eps) / 2, W(np.finfo(dt).smallest_subnormal) / 2)
+    return loss, t_loss, grad, t + half
+
+
+def check_distill(z, t, tok, temp, w=None):
+    r, acc = z.shape[0], "f8" if z.dtype == np.float64 else "f4"
+    w = np.ones(r, acc) if w is None else w.astype(acc)
+    loss, t_loss, grad, t_grad = distill(z, t, tok, temp, w)
+    within(dpt.distill_topk(dev(z), dev(t), dev(tok), temperature=temp), loss, t_loss, "loss")
+    got, dz = dpt.distill_topk_grad(dev(z), dev(t), dev(tok), dev(w), temperature=temp)
+    within(got, loss, t_loss, "loss with gradient")
+    within(dz, grad, t_grad, "gradient")
+
+
+FAR = {"f2": [65504, -65504, 1, 0], "f4": [1e10, -1e10, 1e12, -1e30, 1e38, "max", "min", 0],
+       "f8": [1e10, 1e19, -1e19, -1e100, 1e308, "max", "min", 0]}
+
+
+def far_values(dt):
+    return [dict(max=np.finfo(dt).max, min=np.finfo(dt).min).get(x, x) for x in FAR[dt]]
+
+
+# rows owned by a block (the vocabulary held in registers or read twice) and rows split over blocks
+@pytest.mark.parametrize("temp", [0.7, 1.0, 2.0])
+@pytest.mark.parametrize("dt,v,least", [("f4", 40, 1), ("f4", 1001, 1), ("f4", 20011, 1), ("f4", 100003, 1), ("f4", 90200, 66),
+                                        ("f8", 40, 1), ("f8", 9001, 1), ("f8", 12001, 1), ("f8", 20001, 1),
+                                        ("f2", 40, 1), ("f2", 100003, 1)])
+def test_distill_of_large_finite_values(dt, v, least, temp):
+    rng = np.random.default_rng(v)
+    tdt = "f8" if dt == "f8" else "f4"
+    zs, ts = far_values(dt), far_values(tdt)
+    k, cases = 9, [(a, b) for a in zs + [None] for b in ts + [None]]
+    if v > 5000:  # every value on each side, not every pair
+        cases = [(a, ts[i % len(ts)]) for i, a in enumerate(zs)] + [(None, b) for b in ts] + [(a, None) for a in zs]
+    cases = (cases * (least // len(cases) + 1))[:max(least, len(cases))]
+    r = len(cases)
+    z, t = np.empty((r, v), dt), np.empty((r, k), tdt)
+    tok = np.stack([rng.permutation(v)[:k] for _ in range(r)]).astype("i4")
+    tok[::3, 4] = tok[::3, 1]
+    tok[1::4, 6:] = -1
+    for i, (a, b) in enumerate(cases):
+        z[i] = rng.standard_normal(v) if a is None else a
+        t[i] = 3 * rng.standard_normal(k) if b is None else b
+        if a is not None and i % 2:  # half of the vocabulary so far below that it has no part
+            z[i, rng.random(v) < 0.5] = -a if a > 0 else a if a == np.finfo(dt).min else 1.5 * a
+        if b is not None and i % 3 == 2:
+            t[i, 2] = -b if b > 0 else b
+    check_distill(z, t, tok, temp, rng.uniform(0.5, 2, r))
+
+
+@pytest.mark.parametrize("dt,far,step", [("f4", 1e10, 1024.0), ("f4", -3e12, 2.0 ** 18), ("f8", -1e19, 2048.0), ("f8", 1e40, 2.0 ** 80)])
+@pytest.mark.parametrize("v", [300, 33001, 100003])
+def test_distill_of_far_offsets_at_high_temperatures(dt, far, step, v):
+    """Logits a few steps of their type apart, at temperatures that make something of the steps: on both sides of the limit
+    between the two forms of the exponential."""
+    rng = np.random.default_rng(v)
+    z = (np.dtype(dt).type(far) - step * rng.integers(0, 9, (3, v))).astype(dt)
+    t = (np.dtype(dt).type(far) - step * rng.integers(0, 9, (3, 12))).astype(dt)
+    tok = np.stack([rng.permutation(v)[:12] for _ in range(3)])
+    for temp in (step / 3, step * 2, step * 300):
+        check_distill(z, t, tok, temp)
+
+
+@pytest.mark.parametrize("dt", ["f2", "f4", "f8"])
+@pytest.mark.parametrize("v", [60, 100003])
+def test_distill_of_masked_teacher_tokens(dt, v):
+    """A teacher's token that the student has masked with the lowest value: a large loss, not an infinite one."""
+    rng = np.random.default_rng(3)
+    z, tok = rng.standard_normal((4, v)).astype(dt), np.stack([rng.permutation(v)[:5] for _ in range(4)]).astype("i4")
+    t = rng.standard_normal((4, 5)).astype("f8" if dt == "f8" else "f4")
+    z[0, tok[0, 2]] = z[1, tok[1, 0]] = z[1, tok[1, 4]] = np.finfo(dt).min
+    z[2] = np.finfo(dt).min
+    z[2, tok[2, 3]] = 0
+    t[3, 1:] = np.finfo(t.dtype).min
+    for temp in (0.7, 1.0, 2.0):
+        check_distill(z, t, tok, temp)
+
+
+@pytest.mark.parametrize("dt", ["f4", "f8"])
+def test_distill_at_the_ends_of_the_temperatures(dt):
+    rng = np.random.default_rng(5)
+    z = rng.standard_normal((3, 50)).astype(dt)
+    t, tok = z[:, ::-1].copy(), np.arange(50, dtype="i4")[None].repeat(3, 0)
+    for temp in (1e-4, 1e-20, 1e-40) + ((1e-307, 5e-324) if dt == "f8" else ()):
+        check_distill(z, t, tok, temp)
+    for temp in (1e6, 1e25):  # T^2 is beyond float32: the result may be infinite, but is a number
+        loss, dz = dpt.distill_topk_grad(dev(z), dev(t), dev(tok), temperature=temp)
+        assert not np.isnan(host(loss)).any() and np.isfinite(host(dz)).all()
+    tok = np.arange(10, dtype="i4")[None].repeat(3, 0)
+    assert (host(dpt.distill_topk(dev(z), dev(t[:, :10].copy()), dev(tok), temperature=1e25)) > (1e38 if dt == "f4" else 1e49)).all()
+
+
+@pytest.mark.parametrize("dt", ["f2", "f4", "f8"])
+@pytest.mark.parametrize("v", [50, 4097, 100003])
+def test_distill_at_low_temperatures(dt, v):
+    rng = np.random.default_rng(v)
+    tok = np.stack([rng.permutation(v)[:7] for _ in range(3)]).astype("i4")
+    for temp in (0.006, 0.0055, 0.004, 1e-3):
+        z = (temp * rng.standard_normal((3, v))).astype(dt)
+        z[1] = np.clip(z[1], None, 0)
+        t = (3 * temp * rng.standard_normal((3, 7))).astype("f8" if dt == "f8" else "f4")
+        check_distill(z, t, tok, temp)
+        check_distill(z + np.dtype(dt).type(8), t, tok, temp)
+
+
+@pytest.mark.parametrize("dt,far,temp", [("f2", 1.0, 1e-3), ("f4", 1e30, 1.0), ("f8", 1e300, 1.0)])
+@pytest.mark.parametrize("v", [1000, 20011, 100003])
+def test_distill_of_far_rows_in_place(dt, far, temp, v):
+    rng = np.random.default_rng(v)
+    z = np.where(rng.random((3, v)) < 0.5, far, far / 2).astype(dt)
+    z[1] = rng.standard_normal(v)
+    tok = np.stack([rng.permutation(v)[:7] for _ in range(3)]).astype("i4")
+    t = rng.standard_normal((3, 7)).astype("f8" if dt == "f8" else "f4")
+    want = [host(a) for a in dpt.distill_topk_grad(dev(z), dev(t), dev(tok), temperature=temp)]
+    zd = dev(z)
+    got = dpt.distill_topk_grad(zd, dev(t), dev(tok), temperature=temp, out=(None, zd))
+    assert np.array_equal(host(got[0]), want[0]) and np.array_equal(host(zd), want[1])
+    check_distill(z, t, tok, temp)
