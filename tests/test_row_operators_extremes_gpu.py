@@ -176,3 +176,60 @@ def test_distill_of_far_rows_in_place(dt, far, temp, v):
     got = dpt.distill_topk_grad(zd, dev(t), dev(tok), temperature=temp, out=(None, zd))
     assert np.array_equal(host(got[0]), want[0]) and np.array_equal(host(zd), want[1])
     check_distill(z, t, tok, temp)
+
+
+# ---- layer norm ----------------------------------------------------------------------------------------------------
+def check_layer_norm(x, w, b, eps):
+    """The rounded mean m of a row is off by (k + 2) u max|x| at most, k additions in a chain; d = x - m is then as exact as its own
+    size, and the mean of d corrects m up to (k + 3) u mean|d|.  The variance, mean(d^2) - mean(d)^2, is off by (k + 5) u times
+    the sum of the two."""
+    dt, n = x.dtype, x.shape[-1]
+    u, k = W(ref.unit(dt)), W(ref.depth(n))
+    xs = x.astype(W)
+    near = xs - xs[:, :1]  # (exact in these rows, whose mean would lose digits of its own far from zero)
+    mean = xs[:, 0] + near.mean(-1)
+    d = near - near.mean(-1)[:, None]
+    var = (d * d).mean(-1)
+    rstd = 1 / np.sqrt(var + W(eps))
+    h = d * rstd[:, None]
+    y = h * w.astype(W) + b.astype(W)
+    off = (k + 2) * u * np.abs(xs).max(-1)
+    centre = (k + 4) * u * (np.sqrt(var) + off)
+    rel = (k + 6) * u * (var + 2 * off * off) / (var + W(eps)) + 4 * u
+    assert rel.max() < 0.2  # (below, 1 / sqrt(1 + e) is taken as 1 - e / 2 up to its square)
+    t_h = (centre * rstd * (1 + rel))[:, None] + np.abs(h) * (rel + 3 * u)[:, None] + 2 * u * off[:, None] * rstd[:, None]
+    t_y = t_h * np.abs(w) * W(1.01) + 3 * u * (np.abs(h) * np.abs(w) + np.abs(b))
+    half = np.maximum((np.abs(y) + t_y) * W(np.finfo(dt).eps) / 2, W(np.finfo(dt).smallest_subnormal) / 2)
+    got = dpt.layer_norm(dev(x), dev(w), dev(b), eps=eps, stats=True)
+    within(got[0], y, t_y + half, "y")
+    within(got[1], mean, centre + 2 * u * np.abs(mean), "mean")
+    within(got[2], rstd, rstd * rel, "rstd")
+
+
+# rows by lanes of a wave, by a wave, by blocks, with weights out of registers, and longer than the registers
+@pytest.mark.parametrize("dt", ["f2", "f4", "f8"])
+@pytest.mark.parametrize("n", [7, 24, 100, 500, 1000, 3001, 9001, 20003, 40000, 70000])
+def test_layer_norm_far_from_zero(n, dt):
+    rng = np.random.default_rng(n)
+    w, b = (1 + 0.1 * rng.standard_normal(n)).astype(dt), (0.1 * rng.standard_normal(n)).astype(dt)
+    one = lambda c, s=1.0: (c + s * rng.standard_normal(n)).astype(dt)  # noqa: E731
+    if dt == "f2":
+        rows = [one(1000.0, 8.0), one(-30000.0, 100.0), one(3.0), one(0.0)]
+    else:
+        far = 1.0 if dt == "f4" else 1e8
+        rows = [one(1e3 * far), one(-1e4 * far), one(1e5 * far), one(1e4 * far, 100.0), one(0.0), one(0.0)]
+        rows[4][n // 2] = 1e4  # one large channel in the middle, and as the first element
+        rows[5][0] = -1e4
+    check_layer_norm(np.stack(rows), w, b, 1e-5)
+
+
+@pytest.mark.parametrize("dt", ["f2", "f4", "f8"])
+@pytest.mark.parametrize("n", [7, 100, 1000, 3000, 20003, 70000])
+def test_layer_norm_of_constant_rows(n, dt):
+    w, b = np.ones(n, dt), np.zeros(n, dt)
+    row = lambda *c: np.repeat(np.array(c, dt)[:, None], n, 1)  # noqa: E731
+    check_layer_norm(row(1000.1, 5000.3, -0.1, 0.0, 3.7), w, b, 1e-5)
+    check_layer_norm(row(60000.7, -12345.6), w, b, 1e-3)
+    if dt != "f2":  # the variance of such rows is a rounding error, of either sign: a number all the same
+        y, mean, rstd = (host(a) for a in dpt.layer_norm(dev(row(1e9, -3e12, 1e15 / 3)), stats=True))
+        assert np.isfinite(y).all() and np.isfinite(rstd).all() and (np.abs(mean[:, None] / row(1e9, -3e12, 1e15 / 3) - 1) < 1e-6).all()
