@@ -37,6 +37,7 @@ struct Distill {
     void *loss, *dz;
     void *part; // split rows: [rows][splits] pairs (m, s), then [rows][3 k + 3] values of the teacher's side
     int64_t v, chunk;
+    int64_t row0; // first row of the launch
     int32_t k, tok64, splits;
     int32_t table; // gradient: size of the token table
     double temp;
@@ -310,7 +311,7 @@ __global__ __launch_bounds__(BT, HELD > 8 ? 4 : GRAD ? 6 : 8) void distill_row_k
     __shared__ TeacherSum<A> teacher;
     A *p = (A *)raw, *zk = p + a.k;
     int32_t *token = (int32_t *)(zk + a.k);
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.row0 + blockIdx.x;
     const int tid = (int)threadIdx.x;
     const A c = scale_of<A>(a);
     const T *z = (const T *)a.z + a.map.template off<0>(row);
@@ -510,7 +511,6 @@ template <class T, bool GRAD> __global__ __launch_bounds__(GRAD ? DST_BLOCK : 64
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-constexpr int64_t MAX_GRID = 0x7fffffff;
 constexpr int MAX_K = 2048; // the teacher's entries of a row are held in LDS
 
 struct DistillPlan {
@@ -548,17 +548,20 @@ int64_t distill_workspace(const dpx_array_view *z, int64_t k)
     return splits ? rows * (splits * 2 + 3 * k + 3) * itemsize_of(acc_dtype(z->dtype)) : 0;
 }
 
-template <class T, class TT, bool GRAD, Form FORM> int distill_launch(const Distill &a, hipStream_t s)
+template <class T, class TT, bool GRAD, Form FORM> int distill_launch(Distill &a, hipStream_t s)
 {
     using A = acc_of<T>;
     constexpr int E = 16 / (int)sizeof(T);
     const size_t lds = (size_t)a.k * (2 * sizeof(A) + 4) + (size_t)a.table * 4;
-    const dim3 rows((unsigned)a.map.rows);
     if (a.splits == 0) {
         const int64_t packs = (a.v + E - 1) / E;
         using std::integral_constant;
         auto run = [&](auto bt, auto held) {
-            hipLaunchKernelGGL((distill_row_kernel<T, TT, decltype(bt)::value, decltype(held)::value, GRAD, FORM>), rows, dim3(bt), lds, s, a);
+            in_launches(a.map.rows, 1, bt, [&](int64_t first, int64_t rows) {
+                a.row0 = first;
+                hipLaunchKernelGGL((distill_row_kernel<T, TT, decltype(bt)::value, decltype(held)::value, GRAD, FORM>),
+                                   dim3((unsigned)rows), dim3(bt), lds, s, a);
+            });
         };
         if constexpr (FORM == FAR && sizeof(T) == 2) run(integral_constant<int, 512>{}, integral_constant<int, 0>{}); // (rare)
         else if constexpr (GRAD) {
@@ -577,7 +580,7 @@ template <class T, class TT, bool GRAD, Form FORM> int distill_launch(const Dist
     else {
         hipLaunchKernelGGL((distill_split_kernel<T, TT, GRAD, FORM>), dim3((unsigned)(a.map.rows * (a.splits + 1))), dim3(DST_BLOCK), lds, s, a);
         if constexpr (GRAD) hipLaunchKernelGGL((distill_join_kernel<T, true>), dim3((unsigned)(a.map.rows * a.splits)), dim3(DST_BLOCK), 0, s, a);
-        else hipLaunchKernelGGL((distill_join_kernel<T, false>), rows, dim3(64), 0, s, a);
+        else hipLaunchKernelGGL((distill_join_kernel<T, false>), dim3((unsigned)a.map.rows), dim3(64), 0, s, a);
     }
     const hipError_t rc = hipGetLastError();
     return rc == hipSuccess ? DPX_OK : fail_hip(rc, "distill_topk launch");
@@ -611,7 +614,6 @@ int distill_call(const char *fn, const dpx_array_view *logits, const dpx_array_v
     if (k > MAX_K) return fail(DPX_ERR_BAD_ARGUMENT, f + "at most " + std::to_string(MAX_K) + " teacher entries per row");
     if (a.map.rows == 0) return DPX_OK;
     const DistillPlan pl = distill_plan(a.map.rows, a.v, dt == DPX_DOUBLE, grad);
-    if (a.map.rows * (pl.splits + 1) > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, f + "too many rows for one launch");
     const size_t need = (size_t)distill_workspace(logits, k);
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return fail(DPX_ERR_BAD_ARGUMENT, f + "a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed");

@@ -23,6 +23,7 @@ struct Logits {
     const void *z, *prompt, *output, *plen, *olen, *rep, *freq, *pres, *btok, *bval, *mask;
     void *out;
     int64_t v;
+    int64_t row0;       // first row of the launch
     int64_t np, no, nb; // entries per row
     int32_t steps, groups; // a row's steps (a pack per thread of a block each), and blocks that share them
     int32_t tok64, btok64;
@@ -140,8 +141,9 @@ template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void l
     __shared__ int bias_at[BIAS_LIST];
     __shared__ float bias[BIAS_LIST];
     __shared__ int bias_count;
-    const int64_t row = blockIdx.x / (uint32_t)a.groups;
-    const int group = (int)(blockIdx.x - (uint32_t)row * (uint32_t)a.groups), tid = (int)threadIdx.x, v = (int)a.v;
+    const uint32_t r = blockIdx.x / (uint32_t)a.groups;
+    const int64_t row = a.row0 + r;
+    const int group = (int)(blockIdx.x - r * (uint32_t)a.groups), tid = (int)threadIdx.x, v = (int)a.v;
     const T *z = (const T *)a.z + a.map.template off<L_Z>(row);
     T *out = (T *)a.out + a.map.template off<L_OUT>(row);
     const uint8_t *mask = a.mask ? (const uint8_t *)((const uint32_t *)a.mask + a.map.template off<L_MASK>(row)) : nullptr;
@@ -280,16 +282,16 @@ template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void l
     }
 }
 
-constexpr int64_t MAX_GRID = 0x7fffffff;
-
 template <class T, int CHUNK, int BT> int logits_launch_as(Logits &a, int64_t slots, hipStream_t s)
 {
     constexpr int64_t STEP = BT * (16 / (int)sizeof(T));
     const int64_t span = a.v + 128 / (int64_t)sizeof(T) - 1; // packs may start before the row
     a.steps = (int32_t)((span + STEP - 1) / STEP);
     a.groups = (int32_t)std::max<int64_t>(1, std::min<int64_t>((span + CHUNK - 1) / CHUNK, slots / a.map.rows));
-    if (a.map.rows * a.groups > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, "process_logits: too many rows for one launch");
-    hipLaunchKernelGGL((logits_kernel<T, CHUNK, BT>), dim3((unsigned)(a.map.rows * a.groups)), dim3(BT), 0, s, a);
+    in_launches(a.map.rows, a.groups, BT, [&](int64_t first, int64_t rows) {
+        a.row0 = first;
+        hipLaunchKernelGGL((logits_kernel<T, CHUNK, BT>), dim3((unsigned)(rows * a.groups)), dim3(BT), 0, s, a);
+    });
     const hipError_t rc = hipGetLastError();
     return rc == hipSuccess ? DPX_OK : fail_hip(rc, "process_logits launch");
 }

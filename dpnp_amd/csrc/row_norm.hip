@@ -459,14 +459,14 @@ template <class T, class W, int BT> __global__ __launch_bounds__(BT) void norm_g
 // dw and db of such rows: a second reading, by columns and in a launch before that of dx.  A lane per pack, the block's waves share
 // the rows of its split, whose sums go to a slice of the workspace.  (The sums kept in the workspace by the blocks that walk
 // down the rows: 842 us a call for 3051 x 32768 float16 instead of 227, 302 for 1525 x 16384 float64 instead of 216.)
-template <class T, int BT> __global__ __launch_bounds__(BT) void norm_grad_split_kernel(NormBwd a, int splits)
+template <class T, int BT> __global__ __launch_bounds__(BT) void norm_grad_split_kernel(NormBwd a, int splits, uint32_t block0)
 {
     using A = acc_of<T>;
     constexpr int E = 16 / (int)sizeof(T), NW = BT / 64, U = 4;
     __shared__ A lds[NW][2][E][64];
     const int64_t n = a.n;
-    const uint32_t strips = (uint32_t)((n + 64 * E - 1) / (64 * E)), split = blockIdx.x / strips;
-    const int64_t left = (int64_t)(blockIdx.x - split * strips) * 64 * E;
+    const uint32_t strips = (uint32_t)((n + 64 * E - 1) / (64 * E)), block = block0 + blockIdx.x, split = block / strips;
+    const int64_t left = (int64_t)(block - split * strips) * 64 * E;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int begin = (int)(a.map.rows * split / splits), end = (int)(a.map.rows * (split + 1) / splits);
     auto base_of = [&](int l) { return left + (int64_t)l * E + E <= n ? left + (int64_t)l * E : n - E; };
@@ -512,11 +512,12 @@ template <class T, int BT> __global__ __launch_bounds__(BT) void norm_grad_split
 // loads at a time.
 constexpr int FOLD_COLS = 32, FOLD_ROWS = 16, FOLD_U = 16;
 template <class W, class A>
-__global__ __launch_bounds__(FOLD_COLS *FOLD_ROWS) void norm_grad_fold_kernel(const A *part, int64_t blocks, int64_t n, W *dw, W *db)
+__global__ __launch_bounds__(FOLD_COLS *FOLD_ROWS) void norm_grad_fold_kernel(const A *part, int64_t blocks, int64_t n, W *dw, W *db,
+                                                                                   uint32_t block0)
 {
     __shared__ A lds[FOLD_ROWS][FOLD_COLS + 1];
     const int c = threadIdx.x % FOLD_COLS, r = threadIdx.x / FOLD_COLS;
-    const int64_t col = (int64_t)blockIdx.x * FOLD_COLS + c; // over the 2 n columns of dw and db
+    const int64_t col = (int64_t)(block0 + blockIdx.x) * FOLD_COLS + c; // over the 2 n columns of dw and db
     A s = 0;
     if (col < 2 * n)
         for (int64_t k = r; k < blocks; k += FOLD_ROWS * FOLD_U) {
@@ -724,7 +725,9 @@ template <class T, class W> int norm_grad_launch(NormBwd &a, hipStream_t s)
             if (a.dw) {
                 const int64_t strips = (a.n + 64 * E - 1) / (64 * E);
                 if (strips * parts > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, "layer_norm_grad: rows too long");
-                hipLaunchKernelGGL((norm_grad_split_kernel<T, 256>), dim3((unsigned)(strips * parts)), dim3(256), 0, s, a, (int)parts);
+                in_launches(strips * parts, 1, 256, [&](int64_t first, int64_t count) {
+                    hipLaunchKernelGGL((norm_grad_split_kernel<T, 256>), dim3((unsigned)count), dim3(256), 0, s, a, (int)parts, (uint32_t)first);
+                });
             }
             hipLaunchKernelGGL((norm_grad_long_kernel<T, W, 1024>), dim3((unsigned)blocks), dim3(1024), 0, s, a);
         }
@@ -732,8 +735,10 @@ template <class T, class W> int norm_grad_launch(NormBwd &a, hipStream_t s)
     if (a.dw && !columns) {
         const int64_t fold = (2 * a.n + FOLD_COLS - 1) / FOLD_COLS;
         if (fold > MAX_GRID) return fail(DPX_ERR_BAD_ARGUMENT, "layer_norm_grad: rows too long");
-        hipLaunchKernelGGL((norm_grad_fold_kernel<W, A>), dim3((unsigned)fold), dim3(FOLD_COLS * FOLD_ROWS), 0, s, (const A *)a.part,
-                           parts, a.n, (W *)a.dw, (W *)a.db);
+        in_launches(fold, 1, FOLD_COLS * FOLD_ROWS, [&](int64_t first, int64_t count) {
+            hipLaunchKernelGGL((norm_grad_fold_kernel<W, A>), dim3((unsigned)count), dim3(FOLD_COLS * FOLD_ROWS), 0, s,
+                               (const A *)a.part, parts, a.n, (W *)a.dw, (W *)a.db, (uint32_t)first);
+        });
     }
     const hipError_t rc = hipGetLastError();
     return rc == hipSuccess ? DPX_OK : fail_hip(rc, "layer_norm_grad launch");

@@ -69,6 +69,13 @@ int row_map(const char *fn, const RowArg (&args)[NOPS], RowMap<NOPS> &m, char *(
     }
     return DPX_OK;
 }
+// A launch holds fewer than 2^32 threads: what needs more blocks is launched in parts.  f(first, count) for `total` things of
+// `per` blocks of `threads` threads each.
+template <class F> void in_launches(int64_t total, int64_t per, int threads, F &&f)
+{
+    const int64_t most = 0xffffffff / threads / per;
+    for (int64_t first = 0; first < total; first += most) f(first, total - first < most ? total - first : most);
+}
 // an entry point's body: nothing thrown leaves the library
 template <class F> int row_entry(F &&f)
 {

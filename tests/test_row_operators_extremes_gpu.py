@@ -233,3 +233,68 @@ def test_layer_norm_of_constant_rows(n, dt):
     if dt != "f2":  # the variance of such rows is a rounding error, of either sign: a number all the same
         y, mean, rstd = (host(a) for a in dpt.layer_norm(dev(row(1e9, -3e12, 1e15 / 3)), stats=True))
         assert np.isfinite(y).all() and np.isfinite(rstd).all() and (np.abs(mean[:, None] / row(1e9, -3e12, 1e15 / 3) - 1) < 1e-6).all()
+
+
+# ---- more blocks than one launch holds (2^32 threads) --------------------------------------------------------------------
+def many(a, times):
+    """The rows of `a` over and over: (times, rows, width) without a copy."""
+    return dpt.broadcast_to(dev(a), (times,) + a.shape)
+
+
+def all_equal(got, want):
+    got = host(got)
+    assert got.shape[1:] == want.shape
+    for i in range(0, len(got), 1 << 18):
+        assert (got[i:i + (1 << 18)] == want).all(), i
+
+
+@pytest.mark.parametrize("lists", [False, True])
+def test_logits_of_more_rows_than_a_launch(lists):
+    rng = np.random.default_rng(1)
+    z = rng.standard_normal((13, 8)).astype("f2")
+    times = 2 ** 23 // 13 + 1  # 512 threads a row
+    allowed = rng.integers(1, 255, (13, 1)).astype("u4")
+    tok = rng.integers(0, 8, (13, 3)).astype("i4")
+    kw = lambda f: dict(allowed=f(allowed), **(dict(output_tokens=f(tok), presence_penalty=0.5) if lists else {}))  # noqa: E731
+    want = host(dpt.process_logits(dev(z), **kw(dev)))
+    out = dpt.full((times, 13, 8), 7, dtype="f2")
+    dpt.process_logits(many(z, times), out=out, **kw(lambda a: many(a, times)))
+    all_equal(out, want)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_distill_of_more_rows_than_a_launch(grad):
+    rng = np.random.default_rng(2)
+    z, t = rng.standard_normal((13, 4)).astype("f2"), rng.standard_normal((13, 2)).astype("f4")
+    tok = np.stack([rng.permutation(4)[:2] for _ in range(13)]).astype("i4")
+    times = 2 ** (25 if grad else 24) // 13 + 1  # 128 and 256 threads a row
+    want = [host(a) for a in dpt.distill_topk_grad(dev(z), dev(t), dev(tok))]
+    loss = dpt.full((times, 13), 7, dtype="f4")
+    args = [many(a, times) for a in (z, t, tok)]
+    if grad:
+        dz = dpt.full((times, 13, 4), 7, dtype="f2")
+        dpt.distill_topk_grad(*args, out=(loss, dz))
+        all_equal(dz, want[1])
+    else:
+        want[0] = host(dpt.distill_topk(dev(z), dev(t), dev(tok)))
+        dpt.distill_topk(*args, out=loss)
+    all_equal(loss, want[0])
+
+
+def test_layer_norm_grad_of_more_columns_than_a_launch():
+    rng = np.random.default_rng(3)
+    n = 2 ** 27 + 37  # the fold of the parameters' gradients: 512 threads for 32 columns
+    x, dy = (np.resize(rng.standard_normal(65537).astype("f2"), (1, n)) for _ in range(2))
+    mean, rstd = np.array([0.25], "f4"), np.array([2.0], "f4")
+    out = (None, dpt.full(n, 7, dtype="f2"), dpt.full(n, 7, dtype="f2"))
+    dx, dw, db = dpt.layer_norm_grad(dev(dy), dev(x), dev(mean), dev(rstd), dpt.ones(n, dtype="f2"), out=out)
+    dw, db = host(dw), host(db)
+    assert np.array_equal(db, dy[0])
+    for i in range(0, n, 1 << 24):
+        at = slice(i, i + (1 << 24))
+        # one product of two roundings, rounded to float16 (h is exact but for the rounding of its difference)
+        want = (x[0, at].astype("f8") - 0.25) * 2 * dy[0, at]
+        tol = 2.0 ** -22 * np.abs(want) + np.maximum(np.abs(want) * 2.0 ** -11 * (1 + 2.0 ** -20), 2.0 ** -25)
+        assert (np.abs(dw[at] - want) <= tol).all(), i
+    del dw, db
+    assert np.isfinite(host(dx[:, -65537:])).all()
