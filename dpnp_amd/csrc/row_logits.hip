@@ -32,7 +32,7 @@ struct Logits {
 
 // A token's word in LDS: how often the output holds it, whether the prompt does, whether it has a bias.
 constexpr uint32_t COUNT = (1u << 30) - 1, SEEN_PROMPT = 1u << 31, HAS_BIAS = 1u << 30;
-constexpr int BIAS_LIST = 256; // biases of one chunk that are kept in LDS
+constexpr int FEW_BIASES = 256; // per row; more of them are added up in a sum per token of the chunk
 
 DPX_D int64_t entry_at(const void *p, int is64, int64_t i)
 {
@@ -127,20 +127,73 @@ template <class T, int E> DPX_D void keep_allowed(pack<T, E> &x, uint32_t bits)
     x = u.p;
 }
 
+// The sums of a chunk's biases, made by one wave: 64 entries of the row's list at a time, in their order.  A sum lies at its token
+// (DENSE), or few sums lie one after the other and a byte per token says where.  Entries of one token among the 64 are found by
+// all of them writing their lane to the sum's owner byte: where one does not read itself again, the token's entries are added up
+// one after the other, all others at once.  The work goes with the list, whatever is in it, and a token's sum does not depend on
+// how the lanes get there.
+template <class A, int CHUNK, bool DENSE> struct BiasSums {
+    static constexpr int SUMS = DENSE ? CHUNK : FEW_BIASES;
+    A sum[SUMS];
+    uint8_t owner[SUMS];
+    uint8_t at[DENSE ? 4 : CHUNK];
+    DPX_D A of(int t) const { return sum[DENSE ? t : at[t]]; }
+    static DPX_D void wave_sync() // (a wave's LDS accesses are done in order)
+    {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+    }
+    // lane's entry: token t of the chunk where `in`; `used`: sums so far
+    DPX_D void add(uint32_t *word, int lane, bool in, int t, float value, int &used)
+    {
+        if (__builtin_amdgcn_ballot_w64(in) == 0) return;
+        const bool fresh = in && !(atomicOr(&word[t], HAS_BIAS) & HAS_BIAS); // one lane per token that is new
+        int k = t;
+        if constexpr (!DENSE) {
+            const uint64_t who = __builtin_amdgcn_ballot_w64(fresh);
+            k = used + __builtin_popcountll(who & (((uint64_t)1 << lane) - 1));
+            if (fresh) at[t] = (uint8_t)k;
+            used += __builtin_popcountll(who);
+        }
+        if (fresh) sum[k] = 0;
+        wave_sync();
+        if (!DENSE && in) k = at[t];
+        if (in) owner[k] = (uint8_t)lane;
+        wave_sync();
+        bool alone = in;
+        const bool lost = in && owner[k] != (uint8_t)lane;
+        if (__builtin_amdgcn_ballot_w64(lost) != 0) {
+            wave_sync();
+            if (lost) owner[k] = 255;
+            wave_sync();
+            alone = in && owner[k] != 255;
+            uint64_t todo = __builtin_amdgcn_ballot_w64(in && !alone);
+            while (todo) {
+                const int first = __builtin_ctzll(todo), sum_k = lane_get(k, first);
+                uint64_t same = __builtin_amdgcn_ballot_w64(in && k == sum_k);
+                todo &= ~same;
+                A s = sum[sum_k];
+                for (; same; same &= same - 1) s += (A)lane_get(value, __builtin_ctzll(same));
+                if (lane == first) sum[sum_k] = s;
+            }
+        }
+        if (alone) sum[k] += (A)value;
+        wave_sync();
+    }
+};
+
 // A block takes a run of a row's steps, CHUNK neighbouring tokens at a time, the next chunk's logits on their way.  Per chunk
 // the lists' tokens are counted in LDS words; then every thread looks at the words of its own packs, and where there are any,
 // puts the pack into its place in LDS and processes the named tokens there one by one (a wave runs as many rounds as the most
 // named pack of its lanes has, mostly one), clears the words, and stores the pack.
-template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void logits_kernel(Logits a)
+template <class T, int CHUNK, int BT, bool DENSE> __global__ __launch_bounds__(BT, 6) void logits_kernel(Logits a)
 {
     using A = acc_of<T>;
     constexpr int E = 16 / (int)sizeof(T), PPT = CHUNK / (BT * E);
     static_assert(PPT * BT * E == CHUNK && CHUNK % 32 == 0 && CHUNK <= 65536);
     __shared__ __attribute__((aligned(16))) uint32_t word[CHUNK];
     __shared__ __attribute__((aligned(16))) T value[BT * E]; // a pack per thread
-    __shared__ int bias_at[BIAS_LIST];
-    __shared__ float bias[BIAS_LIST];
-    __shared__ int bias_count;
+    __shared__ BiasSums<A, CHUNK, DENSE> biases;
     const uint32_t r = blockIdx.x / (uint32_t)a.groups;
     const int64_t row = a.row0 + r;
     const int group = (int)(blockIdx.x - r * (uint32_t)a.groups), tid = (int)threadIdx.x, v = (int)a.v;
@@ -204,29 +257,27 @@ template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void l
             __syncthreads(); // the words are clear
             prompt.take(begin, n, [&](int t) { atomicOr(&word[t], SEEN_PROMPT); });
             output.take(begin, n, [&](int t) { atomicAdd(&word[t], 1u); });
-            if (a.btok && lane >= 0) { // the chunk's biases, listed in their order
-                int count = 0;
-                for (int k = lane; k - lane < nb; k += 64) {
-                    int token = b_token;
-                    float value = b_value;
-                    if (k >= 64) {
-                        token = k < nb ? bias_token(k) : TokenScan<BT>::NONE;
-                        value = k < nb ? bias_value(k) : 0.0f;
+            if (a.btok && lane >= 0) { // the chunk's biases
+                constexpr int B = DENSE ? 4 : 1; // rounds of 64 entries that are sent for together
+                int used = 0, token[B];
+                float value[B];
+                token[0] = b_token, value[0] = b_value;
+                for (int k0 = 0; k0 < nb; k0 += 64 * B) {
+#pragma unroll
+                    for (int q = 0; q < B; ++q) {
+                        const int k = k0 + q * 64 + lane;
+                        if (k0 + q == 0) continue;
+                        token[q] = k < nb ? bias_token(k) : TokenScan<BT>::NONE;
+                        value[q] = k < nb ? bias_value(k) : 0.0f;
                     }
-                    const uint32_t t = (uint32_t)token - (uint32_t)begin;
-                    const bool in = t < (uint32_t)n;
-                    const uint64_t who = __builtin_amdgcn_ballot_w64(in);
-                    const int at = count + __builtin_popcountll(who & (((uint64_t)1 << lane) - 1));
-                    if (in) {
-                        atomicOr(&word[t], HAS_BIAS);
-                        if (at < BIAS_LIST) {
-                            bias_at[at] = (int)t;
-                            bias[at] = value;
-                        }
+#pragma unroll
+                    for (int q = 0; q < B; ++q) {
+                        const uint32_t t = (uint32_t)token[q] - (uint32_t)begin;
+                        asm volatile("" : "+v"(value[q])); // (arrived: a load left pending where no entry is in the chunk would be
+                                                           // waited for, and every other with it, by whoever has its register next)
+                        biases.add(word, lane, t < (uint32_t)n, (int)t, value[q], used);
                     }
-                    count += __builtin_popcountll(who);
                 }
-                if (lane == 0) bias_count = count;
             }
             __syncthreads();
         }
@@ -250,17 +301,7 @@ template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void l
                         if (word_e & (SEEN_PROMPT | COUNT)) r = r > 0 ? r / rep : r * rep;
                         const uint32_t said = word_e & COUNT;
                         if (said) r = (r - freq * (A)said) - pres;
-                        if (word_e & HAS_BIAS) { // the biases of this token added up in their order, then to the logit
-                            A s = 0;
-                            if (bias_count <= BIAS_LIST) {
-                                for (int k = 0; k < bias_count; ++k)
-                                    if (bias_at[k] == i + e) s += (A)bias[k];
-                            }
-                            else
-                                for (int k = 0; k < nb; ++k)
-                                    if (bias_token(k) == begin + i + e) s += (A)bias_value(k);
-                            r += s;
-                        }
+                        if (a.btok && (word_e & HAS_BIAS)) r += biases.of(i + e);
                         mine[e] = (T)r;
                         word[i + e] = 0;
                     }
@@ -282,7 +323,7 @@ template <class T, int CHUNK, int BT> __global__ __launch_bounds__(BT, 6) void l
     }
 }
 
-template <class T, int CHUNK, int BT> int logits_launch_as(Logits &a, int64_t slots, hipStream_t s)
+template <class T, int CHUNK, int BT, bool DENSE> int logits_launch_as(Logits &a, int64_t slots, hipStream_t s)
 {
     constexpr int64_t STEP = BT * (16 / (int)sizeof(T));
     const int64_t span = a.v + 128 / (int64_t)sizeof(T) - 1; // packs may start before the row
@@ -290,7 +331,7 @@ template <class T, int CHUNK, int BT> int logits_launch_as(Logits &a, int64_t sl
     a.groups = (int32_t)std::max<int64_t>(1, std::min<int64_t>((span + CHUNK - 1) / CHUNK, slots / a.map.rows));
     in_launches(a.map.rows, a.groups, BT, [&](int64_t first, int64_t rows) {
         a.row0 = first;
-        hipLaunchKernelGGL((logits_kernel<T, CHUNK, BT>), dim3((unsigned)(rows * a.groups)), dim3(BT), 0, s, a);
+        hipLaunchKernelGGL((logits_kernel<T, CHUNK, BT, DENSE>), dim3((unsigned)(rows * a.groups)), dim3(BT), 0, s, a);
     });
     const hipError_t rc = hipGetLastError();
     return rc == hipSuccess ? DPX_OK : fail_hip(rc, "process_logits launch");
@@ -301,6 +342,10 @@ template <class T, int CHUNK, int BT> int logits_launch_as(Logits &a, int64_t sl
 // nothing in flight meanwhile: 38.7; 4096 tokens by 256 threads: 30.3).  Without lists there is nothing to keep: a block per
 // chunk streams better (mask alone 22.8 against 24.8 us).  With few rows small chunks, so that the row is spread over the CUs
 // (1 row of 131072 float32, lists of 700 and 300 tokens: 5.6 us).
+// Biases: up to 256 a row in few sums, more in a sum per token, which costs LDS and with it half of the chunk (256 rows of
+// 100003 float16 with 50 / 256 of them: 27.0 / 34.4 us, 29.6 / 40.4 with a sum per token; rows of 1000 the same either way).  One
+// wave goes through the list for each chunk: 64 rows of 1000 float32 with 300 biases 10.8 us, one row of 16000 with as many
+// biases 111, of 131072 with as many 690; 256 rows of 100003 float16 with 2000 155.
 // Letting the threads that hold a token process it in LDS, instead of the thread that holds the logit: 28.4 and 6.4 us
 // (one more barrier), 44 against 50 for 1024 rows of 32000, where one token in 13 is named.
 template <class T> int logits_launch(Logits &a, hipStream_t s)
@@ -308,8 +353,10 @@ template <class T> int logits_launch(Logits &a, hipStream_t s)
     constexpr int E = 16 / (int)sizeof(T), CHUNK = 512 * E * (sizeof(T) == 4 ? 3 : 2);
     const int64_t cus = device_cus(), many = (int64_t)1 << 40;
     const bool lists = a.prompt || a.output || a.btok;
-    if (a.map.rows * ((a.v + CHUNK - 1) / CHUNK) >= cus * 2) return logits_launch_as<T, CHUNK, 512>(a, lists ? cus * 3 : many, s);
-    return logits_launch_as<T, 256 * E, 256>(a, many, s);
+    const bool full = a.map.rows * ((a.v + CHUNK - 1) / CHUNK) >= cus * 2;
+    if (a.btok && a.nb > FEW_BIASES)
+        return full ? logits_launch_as<T, 512 * E, 512, true>(a, cus * 3, s) : logits_launch_as<T, 256 * E, 256, true>(a, many, s);
+    return full ? logits_launch_as<T, CHUNK, 512, false>(a, lists ? cus * 3 : many, s) : logits_launch_as<T, 256 * E, 256, false>(a, many, s);
 }
 
 int process_logits_call(const dpx_array_view *logits, const dpx_logits_args *g, const dpx_array_view *out, hipStream_t stream)

@@ -298,3 +298,71 @@ def test_layer_norm_grad_of_more_columns_than_a_launch():
         assert (np.abs(dw[at] - want) <= tol).all(), i
     del dw, db
     assert np.isfinite(host(dx[:, -65537:])).all()
+
+
+# ---- biases of logits ------------------------------------------------------------------------------------------------
+def biased(z, tok, val):
+    """Each token's biases added up in their order in the type of the sums, then to the logit."""
+    acc = "f8" if z.dtype == np.float64 else "f4"
+    s = np.zeros(z.shape, acc)
+    inside = (tok >= 0) & (tok < z.shape[1])
+    np.add.at(s, (np.arange(len(z))[:, None].repeat(tok.shape[1], 1)[inside], tok[inside]), val.astype(acc)[inside])
+    return (z.astype(acc) + s).astype(z.dtype)
+
+
+@pytest.mark.parametrize("dt,itype", [("f2", "i4"), ("f4", "i4"), ("f4", "i8"), ("f8", "i8")])
+@pytest.mark.parametrize("rows,v", [(2, 40), (3, 1000), (2, 20011), (600, 1000), (40, 100003)])
+@pytest.mark.parametrize("nb", [1, 63, 64, 65, 130, 256, 257, 300, 1000, 4099])
+def test_logits_biases_in_their_order(rows, v, nb, dt, itype):
+    if rows * nb > 700000:
+        rows = 520
+    rng = np.random.default_rng(nb)
+    z = rng.standard_normal((rows, v)).astype(dt)
+    val = rng.uniform(-3, 3, (rows, nb)).astype("f4")
+    tok = rng.integers(-2, v + 2, (rows, nb))
+    tok[0] = v - 1                                          # one token only
+    if rows > 2:
+        tok[1] = rng.integers(0, 3, nb) * (v // 3)          # few of them
+        tok[2] = np.arange(nb) % v                          # neighbours
+    if rows > 4:
+        tok[3, ::2] = tok[3, 0] % v                         # one token between others
+        tok[4] = np.where(rng.random(nb) < 0.5, -1, tok[4])
+    tok = tok.astype(itype)
+    got = host(dpt.process_logits(dev(z), bias_tokens=dev(tok), bias_values=dev(val)))
+    assert np.array_equal(got, biased(z, tok, val))
+
+
+def test_logits_biases_beside_everything_else():
+    rng = np.random.default_rng(7)
+    for rows, v, nb in ((3, 1000, 300), (520, 700, 300), (3, 30000, 5000)):
+        z = rng.standard_normal((rows, v)).astype("f4")
+        tok, val = rng.integers(-2, v + 2, (rows, nb)).astype("i4"), rng.integers(-40, 41, (rows, nb)).astype("f4") / 4
+        said = rng.integers(-2, v + 2, (rows, 200)).astype("i4")
+        allowed = rng.integers(0, 2 ** 32, (rows, (v + 31) // 32), dtype="u8").astype("u4")
+        want, tol, _ = ref.process_logits(z, prompt=said[:, :100], output=said, rep=1.5, freq=0.25, pres=0.5, btok=tok, bval=val,
+                                          allowed=allowed)
+        got = host(dpt.process_logits(dev(z), prompt_tokens=dev(said[:, :100].copy()), output_tokens=dev(said), repetition_penalty=1.5,
+                                      frequency_penalty=0.25, presence_penalty=0.5, bias_tokens=dev(tok), bias_values=dev(val),
+                                      allowed=dev(allowed)))
+        masked = want == -np.inf
+        assert (got[masked] == -np.inf).all() and (np.abs(got[~masked] - want[~masked]) <= tol[~masked]).all()
+
+
+def test_logits_time_goes_with_the_number_of_biases():
+    import time
+    rng = np.random.default_rng(9)
+    v = 16000
+    z, out = dev(rng.standard_normal((1, v)).astype("f4")), dpt.empty((1, v), dtype="f4")
+
+    def seconds(nb):
+        tok, val = dev(rng.integers(0, v, (1, nb)).astype("i4")), dev(rng.standard_normal((1, nb)).astype("f4"))
+        best = np.inf
+        for _ in range(8):
+            start = time.perf_counter()
+            dpt.process_logits(z, bias_tokens=tok, bias_values=val, out=out)
+            out.sycl_queue.wait()
+            best = min(best, time.perf_counter() - start)
+        return best
+
+    # 16 times as many: about 6 times the time (a call's fixed costs are part of both); every token through the whole list: 200
+    assert seconds(16000) < 50 * seconds(1000)
