@@ -12,7 +12,7 @@ from .. import _lib
 from . import _tensor_impl as ti
 from ._copy_utils import copy
 from ._device import alloc
-from ._dtypes import float32, float64
+from ._dtypes import float16, float32, float64
 from ._manipulation_functions import broadcast_to
 from ._usmarray import usm_ndarray
 
@@ -141,7 +141,8 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, /, *, out=None):
     """Gradients of `layer_norm`: (dx, dweight, dbias) for `grad`, the gradient of its result.
 
     mean, rstd: the statistics that layer_norm(x, ..., stats=True) returned.  dweight and dbias have the type of weight and
-    are None without one.  out: (dx, dweight, dbias) arrays, each may be None; dx may be grad or x itself.
+    are None without one, but for a dbias array given in `out` (of x's type, or float32 for float16 x): the gradient of a bias
+    without a weight beside it.  out: (dx, dweight, dbias) arrays, each may be None; dx may be grad or x itself.
     """
     x = _data(x, "layer_norm_grad", "x")
     grad = _data(grad, "layer_norm_grad", "grad")
@@ -150,12 +151,21 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, /, *, out=None):
     weight = _vector(weight, "weight")
     ox, ow, ob = _several(out, 3, "(dx, dweight, dbias)")
     reads = (grad, x, mean, rstd, weight)
-    if weight is None and (ow is not None or ob is not None):
-        raise ValueError("dweight and dbias need weight")
+    if weight is None and ow is not None:
+        raise ValueError("dweight would need weight")
     dx = _Out(ox, x._shape, x._dtype, "dx", reads, (grad, x))
     if weight is None:
-        _ext.layer_norm_grad(grad, x, mean, rstd, None, dx.kernel, None, None)
-        return dx.done(), None, None
+        if ob is None:
+            _ext.layer_norm_grad(grad, x, mean, rstd, None, dx.kernel, None, None)
+            return dx.done(), None, None
+        shape, dt = x._shape[-1:], x._dtype
+        if dt == float16 and isinstance(ob, usm_ndarray) and ob._dtype == float32:
+            dt = float32
+        db = _Out(ob, shape, dt, "dbias", reads)
+        _apart(dx, db)
+        # (the kernels make both sums)
+        _ext.layer_norm_grad(grad, x, mean, rstd, None, dx.kernel, usm_ndarray._new_contiguous(shape, dt), db.kernel)
+        return dx.done(), None, db.done()
     dw = _Out(ow, weight._shape, weight._dtype, "dweight", reads)
     db = _Out(ob, weight._shape, weight._dtype, "dbias", reads)
     _apart(dx, dw, db)

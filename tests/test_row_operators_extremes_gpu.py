@@ -366,3 +366,24 @@ def test_logits_time_goes_with_the_number_of_biases():
 
     # 16 times as many: about 6 times the time (a call's fixed costs are part of both); every token through the whole list: 200
     assert seconds(16000) < 50 * seconds(1000)
+
+
+# ---- a bias without a weight -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt,bdt", [("f2", "f2"), ("f2", "f4"), ("f4", "f4"), ("f8", "f8")])
+@pytest.mark.parametrize("rows,n", [(1, 5), (5, 100), (130, 1000), (700, 96), (130, 9001), (40, 40000)])
+def test_layer_norm_grad_of_a_bias_alone(rows, n, dt, bdt):
+    rng = np.random.default_rng(n)
+    x, dy = rng.standard_normal((rows, n)).astype(dt), rng.standard_normal((rows, n)).astype(dt)
+    _, mean, rstd = dpt.layer_norm(dev(x), None, dev(np.ones(n, bdt)), stats=True)
+    out = dpt.full(n, 7, dtype=bdt)
+    dx, dw, db = dpt.layer_norm_grad(dev(dy), dev(x), mean, rstd, out=(None, None, out))
+    assert dw is None and db is out
+    # dx and dbias as with a weight of ones of that type
+    want = dpt.layer_norm_grad(dev(dy), dev(x), mean, rstd, dev(np.ones(n, bdt)))
+    assert np.array_equal(host(dx), host(want[0])) and np.array_equal(host(db), host(want[2]))
+    tol = ref.layer_norm_grad_tolerances(dy, x, host(mean), host(rstd), np.ones(n, bdt))[2]
+    within(db, dy.astype(W).sum(0), tol)
+    xd, pair = dev(dy), dpt.full(2 * n, 7, dtype=bdt)  # in place, and into every other element
+    dpt.layer_norm_grad(xd, dev(x), mean, rstd, out=(xd, None, pair[::2]))
+    assert np.array_equal(host(xd), host(dx)) and np.array_equal(host(pair)[::2], host(db)) and (host(pair)[1::2] == 7).all()
+    assert dpt.layer_norm_grad(dev(dy), dev(x), mean, rstd)[1:] == (None, None)
