@@ -85,17 +85,21 @@ template <int G, int BT, int NV, class A> DPX_D void row_sums(A (&v)[NV], SumPar
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------
-// A row's statistics from its rounded mean m and the means of d = x - m and d^2.
+// A row's statistics from its rounded mean m and the means of d = x - m and d^2.  A mean(d) of up to four roundings of the
+// differences is what their own roundings leave and not the mean's error (that of rows about zero is far smaller): it is left out,
+// and so is one that is no number.
 template <class A> struct NormStats {
     A mean, shift, rstd, shift_rstd;
-    DPX_D NormStats(A m, A d, A dd, A eps) : mean(m), shift(d)
+    DPX_D NormStats(A m, A d, A dd, A eps) : mean(m)
     {
-        const A v = row_fma(-d, d, dd);
+        constexpr A u4 = sizeof(A) == 4 ? A(0x1p-22) : A(0x1p-51);
+        shift = d * d > u4 * u4 * dd ? d : A(0);
+        const A v = row_fma(-shift, shift, dd);
         rstd = A(1) / row_sqrt((v < 0 ? A(0) : v) + eps); // (NaN stays)
-        shift_rstd = -d * rstd;
+        shift_rstd = -shift * rstd;
     }
     DPX_D A centred(A x) const { return row_fma(x - mean, rstd, shift_rstd); }
-    DPX_D A whole_mean() const { return shift == shift ? mean + shift : mean; } // (an infinite mean is the mean)
+    DPX_D A whole_mean() const { return mean + shift; }
 };
 template <class T, class W, int E, int PPL, int G, int BT> __global__ __launch_bounds__(BT) void norm_fwd_kernel(NormFwd a)
 {
