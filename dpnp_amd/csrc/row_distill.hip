@@ -19,9 +19,10 @@
 // what does not fit is read again while it is still in a cache.  Few long rows are split over blocks that leave (m, s) in the
 // caller's workspace, and a second launch joins them.
 //
-// Measured (rocprofv3): gradient of 2048 x 65536 float16 101 us (5.3 TB/s; its exponentials and the rest of its arithmetic
+// Measured (rocprofv3): gradient of 2048 x 65536 float16 100 us (5.4 TB/s; its exponentials and the rest of its arithmetic
 // take about 50 us of it, which the loads and stores of the other block of the CU hide only in part), of 513 x 100003
-// float32 82 us (one row more than two rounds of the 256 CUs; 512 rows 75), loss of 2048 x 131072 float16 85 us (6.3 TB/s).
+// float32 84 us (one row more than two rounds of the 256 CUs; 512 rows 75), loss of 2048 x 131072 float16 87 us (6.2 TB/s;
+// with the FAR form 4 more, the gradient 1 to 2 more).
 // Tried and not kept: rows that come in while the gradients of the row before go out (persistent blocks, a held pack's
 // registers reloaded after its last use: 160 us, the row's state no longer fits the registers); packs held in LDS as well
 // (158 us for 513 x 100003); a wave of its own for the teacher's side (a block of 9 waves leaves room for one a CU: 111 us).
@@ -518,11 +519,18 @@ struct DistillPlan {
     int64_t chunk;
 };
 // A block per row is one launch and reads a row once, but a few long rows leave most of the card idle; split rows cost two
-// launches, about 11 us a call.  A call with a block per row / split rows, us (float16 and float32 within 4 us):
-//                            1 row         64 rows       96 rows       128 rows      192 rows
-//   float32  65536 gradient   9.3 / 13.2   13.1 / 14.8   loss 1 row 7.6 / 11.0, 64 rows 10.4 / 11.3
-//           131072 gradient  19.0 / 12.2   21.5 / 20.8   23.3 / 29.0   28.9 / 37.2
-//                  loss      16.0 / 10.7   17.3 / 11.2   18.0 / 15.2   18.4 / 18.5
+// launches, about 11 us a call.  A call with a block per row / split rows, us (the two ways cross at about the same
+// lengths for float16 and float32):
+//                            1 row         64 rows       128 rows         and   1 row         64 rows       128 rows
+//   float16  65536 gradient   9.8 / 11.8   13.8 / 15.7   15.7 / 18.4   loss    7.2 / 10.2    8.3 / 10.1    8.5 / 10.3
+//            90000           12.9 / 11.8   16.9 / 17.6   16.8 / 21.2           8.2 / 10.0   10.7 / 10.1   11.0 / 11.9
+//            98304           13.6 / 11.7   15.7 / 16.1   17.2 / 21.1           8.1 / 10.0   10.8 / 10.1   10.8 / 11.9
+//           131072           14.7 / 11.9   16.7 / 15.7   17.8 / 22.3           9.8 / 10.2   13.1 / 10.2   13.5 / 12.6
+//   float32  65536           10.3 / 11.8   14.6 / 16.6   16.1 / 23.0           7.1 / 10.0    8.6 / 10.1    9.2 / 11.2
+//            90000           14.4 / 11.7   18.4 / 19.9   21.0 / 28.1           9.6 / 10.0   11.0 / 10.2   11.8 / 13.1
+//            98304           15.2 / 11.8   18.1 / 18.7   22.0 / 29.3           9.2 / 10.0   10.9 / 10.1   12.0 / 13.6
+//           131072           19.6 / 11.9   22.4 / 20.6   29.0 / 37.2          11.5 / 10.1   13.7 / 11.0   15.1 / 16.3
+//                            1 row         64 rows                     128 rows      192 rows
 //   float64  12288 gradient  13.9 / 12.2   17.7 / 14.0   loss 1 row  7.5 / 10.2, 64 rows 8.9 / 10.4
 //            16384 gradient  15.6 / 11.6   17.8 / 15.3                 18.8 / 18.3
 //                  loss       9.2 / 10.2   10.0 / 10.6                  9.9 / 11.2

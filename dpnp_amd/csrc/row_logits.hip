@@ -338,7 +338,7 @@ template <class T, int CHUNK, int BT, bool DENSE> int logits_launch_as(Logits &a
 }
 // Chunks and blocks.  With many rows: a chunk of two packs per thread of 512 (float32: three; more spill), three blocks a CU
 // that share out each row's steps and keep the next chunk's logits in flight while they count (256 rows of 100003 float16,
-// lists of 1800 and 700 tokens, 50 biases, mask: 27.9 us, 3.8 TB/s; a block per chunk, which reads the lists anew and has
+// lists of 1800 and 700 tokens, 50 biases, mask: 27.8 us, 3.9 TB/s; a block per chunk, which reads the lists anew and has
 // nothing in flight meanwhile: 38.7; 4096 tokens by 256 threads: 30.3).  Without lists there is nothing to keep: a block per
 // chunk streams better (mask alone 22.8 against 24.8 us).  With few rows small chunks, so that the row is spread over the CUs
 // (1 row of 131072 float32, lists of 700 and 300 tokens: 5.6 us).
@@ -346,8 +346,9 @@ template <class T, int CHUNK, int BT, bool DENSE> int logits_launch_as(Logits &a
 // 100003 float16 with 50 / 256 of them: 27.0 / 34.4 us, 29.6 / 40.4 with a sum per token; rows of 1000 the same either way).  One
 // wave goes through the list for each chunk: 64 rows of 1000 float32 with 300 biases 10.8 us, one row of 16000 with as many
 // biases 111, of 131072 with as many 690; 256 rows of 100003 float16 with 2000 155.
-// Letting the threads that hold a token process it in LDS, instead of the thread that holds the logit: 28.4 and 6.4 us
-// (one more barrier), 44 against 50 for 1024 rows of 32000, where one token in 13 is named.
+// Letting the threads that hold a token process it in LDS, instead of the thread that holds the logit: 28.4 us for the batch and
+// 6.4 for the one row (one more barrier).  Where one token in 13 is named (1024 rows of 32000, 2500 different tokens each) the
+// holders of the logits take 37 us for float16 and 60 for float32, 20 and 40 of it for the bytes.
 template <class T> int logits_launch(Logits &a, hipStream_t s)
 {
     constexpr int E = 16 / (int)sizeof(T), CHUNK = 512 * E * (sizeof(T) == 4 ? 3 : 2);

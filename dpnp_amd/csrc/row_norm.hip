@@ -13,9 +13,10 @@
 // registers.  float16 and float32 rows are computed in float32, float64 rows in float64; every result is rounded once, at
 // its store.
 //
-// Measured (rocprofv3): forward of 16384 x 4096 float16 with float32 parameters 47 us (5.7 TB/s; one block per row that
-// reads the weights anew 60 us, one wave per row 56), 20011 x 1001 float32 29.5 us (5.4 TB/s: rows off the 16-byte grid);
-// backward of 16384 x 4096 float16 79 us + 4.8 for the fold of the column sums (5.1 TB/s), 2049 x 10007 float32 53 + 6.5.
+// Measured (rocprofv3): forward of 16384 x 4096 float16 with float32 parameters 48 us (5.6 TB/s; one block per row that
+// reads the weights anew 60 us, one wave per row 56), 20011 x 1001 float32 30.5 us (5.3 TB/s: rows off the 16-byte grid);
+// backward of 16384 x 4096 float16 80 us + 4.9 for the fold of the column sums (5.0 TB/s), 2049 x 10007 float32 53.5 + 6.6.
+// The sum of d beside that of d^2 costs the forward pass about 1 us of the 48 and 4 of the 118 of 1428 x 70000 float16.
 // The backward's time does not change with the prefetch distance (0, 1, 2 rows), the threads per row (256 to 1024) or its
 // arithmetic (9 against 16 instructions per element): it is what three streams of persistent blocks reach here.
 #include "row_ops.hpp"
@@ -34,7 +35,8 @@ struct NormFwd {
 
 // Lane li's j-th pack of a row: packs lie G apart.  A row's last pack is moved back so that it ends with the row (rows
 // hold at least E elements); its first `skip` elements belong to the pack before.  Packs beyond the row are that last pack
-// again with every element skipped: their loads are harmless and nothing is stored for them.
+// again with every element skipped: they add nothing to a sum, and what is stored for skipped elements is what their own lanes
+// store there, computed from the same values.
 template <int E, int G> struct PackAt {
     int64_t base;
     int skip;
@@ -177,7 +179,7 @@ template <class T, class W, int E, int PPL, int G, int BT> __global__ __launch_b
 }
 
 // Rows too long for a block's registers: blocks of 1024 threads walk down the rows and read each three times (the second and
-// third time from a cache; 1428 x 70000 float16 113 us, element by element 334).
+// third time from a cache; 1428 x 70000 float16 118 us, element by element 334).
 // f(base, skip) for the thread's packs of a row; as in PackAt the last one is moved back.  Only its own elements are stored: a
 // row may be worked on in place.
 template <int E, int BT, class F> DPX_D void each_pack(int64_t n, F f)
@@ -462,7 +464,7 @@ template <class T, class W, int BT> __global__ __launch_bounds__(BT) void norm_g
 }
 // dw and db of such rows: a second reading, by columns and in a launch before that of dx.  A lane per pack, the block's waves share
 // the rows of its split, whose sums go to a slice of the workspace.  (The sums kept in the workspace by the blocks that walk
-// down the rows: 842 us a call for 3051 x 32768 float16 instead of 227, 302 for 1525 x 16384 float64 instead of 216.)
+// down the rows: 842 us a call for 3051 x 32768 float16 instead of 222, 302 for 1525 x 16384 float64 instead of 215.)
 template <class T, int BT> __global__ __launch_bounds__(BT) void norm_grad_split_kernel(NormBwd a, int splits, uint32_t block0)
 {
     using A = acc_of<T>;
@@ -512,7 +514,7 @@ template <class T, int BT> __global__ __launch_bounds__(BT) void norm_grad_split
     }
 }
 
-// dw and db: the blocks' sums added up in a fixed order.  32 columns by 32 threads that each take every 32nd block, eight
+// dw and db: the blocks' sums added up in a fixed order.  32 columns by 16 threads that each take every 16th block, sixteen
 // loads at a time.
 constexpr int FOLD_COLS = 32, FOLD_ROWS = 16, FOLD_U = 16;
 template <class W, class A>

@@ -192,7 +192,8 @@ def distill_topk(logits, teacher_logits, teacher_tokens, /, *, temperature=1.0, 
 def distill_topk_grad(logits, teacher_logits, teacher_tokens, weights=None, /, *, temperature=1.0, out=None):
     """(loss, dlogits): the losses of `distill_topk` and the gradient of sum(weights * loss) by the logits.
 
-    weights (...): the loss's type, None for ones; a row of weight 0 (padding) gets a zero gradient whatever its logits are.
+    weights (...): the loss's type, None for ones; a row of weight 0 (padding) gets a zero gradient whatever its logits are.  Its
+    loss is that of `distill_topk`, NaN where its logits make it so: where(weights != 0, loss, 0) before it is added up.
     out: (loss, dlogits) arrays, each may be None; dlogits may be logits itself.
     """
     logits = _data(logits, "distill_topk_grad", "logits")

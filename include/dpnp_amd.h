@@ -545,7 +545,8 @@ int dpx_distill_topk(const dpx_array_view *logits, const dpx_array_view *teacher
                      const dpx_array_view *teacher_tokens, double temperature, const dpx_array_view *loss, void *workspace,
                      size_t workspace_bytes, void *stream);
 /* The loss and dlogits (may be logits) = the gradient of sum(weights * loss); weights: acc, the rows' shape, NULL for ones.
- * A row of weight 0 and a row with no entry get zeros whatever their logits are. */
+ * A row of weight 0 and a row with no entry get zeros whatever their logits are (the loss of a row of weight 0 is the
+ * loss all the same). */
 int dpx_distill_topk_grad(const dpx_array_view *logits, const dpx_array_view *teacher_logits,
                           const dpx_array_view *teacher_tokens, const dpx_array_view *weights, double temperature,
                           const dpx_array_view *loss, const dpx_array_view *dlogits, void *workspace,
